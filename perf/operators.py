@@ -262,7 +262,7 @@ def _plain_extend(s):
     csum = torch.cumsum(want, 0)
     ok = fits & ((want == 0) | (csum <= count))
     granted = torch.where(ok, new, 0)
-    taken = torch.where(ok, csum, 0).max()
+    taken = torch.where(ok & (want > 0), csum, 0).max()
     j = torch.arange(W, device=table.device)
     fresh = ok[:, None] & (j >= p0[:, None]) & (j < p1[:, None])
     at = count - 1 - (csum - want)[:, None] - (j - p0[:, None])

@@ -22,6 +22,7 @@ class Strides(ctypes.Structure):
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_L = ctypes.c_int64
 _S = Strides
 SIGNATURES = {
     "fa_b200_forward": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P]),
@@ -41,6 +42,16 @@ SIGNATURES = {
     "fa_b200_backward_noalloc": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P,
                                       _I, _I, _I, _I, _I, _I, _P]),
     "fa_b200_backward_noalloc_max_rows": (_SZ, []),
+    "fa_b200_paged_table_workspace_bytes": (_SZ, [_I]),
+    "fa_b200_paged_extend": (_I, [_P, _P, _P, _L, _P, _P, _P, _P, _P, _P, _P, _SZ,
+                                  _I, _I, _I, _I, _I, _P]),
+    "fa_b200_paged_release": (_I, [_P, _P, _P, _L, _P, _P, _P, _P, _P, _SZ,
+                                   _I, _I, _I, _I, _P]),
+    "fa_b200_paged_append": (_I, [_P, _S, _P, _S, _P, _P, _S, _P, _S,
+                                  _I, _I, _I, _I, _I, _I, _P]),
+    "fa_b200_paged_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
+    "fa_b200_paged_attn": (_I, [_P, _S, _P, _S, _P, _S, _P, _L, _P, _P, _S, _P, _P, _SZ,
+                                _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "fa_b200_device_error": (_I, [_I, _I]),
     "fa_b200_device_error_async": (_I, [_P, _P]),
     "fa_b200_debug_tma_check": (_I, [_I, ctypes.POINTER(ctypes.c_ulonglong), _I]),

@@ -27,6 +27,7 @@
 #include "fa_bwd.cuh"
 #include "fa_fwd.cuh"
 #include "fa_fwd_persist.cuh"
+#include "fa_paged.cuh"
 
 namespace fab {
 
@@ -247,6 +248,16 @@ int check_shape(int B, int Hq, int Hkv, int N, int D) {
   if (D != 64 && D != 128) return FA_B200_ERR_HEAD_DIM;
   if (B < 1 || N < 1 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0) return FA_B200_ERR_SHAPE;
   if (N > kMaxN) return FA_B200_ERR_TOO_LARGE;
+  return FA_B200_OK;
+}
+
+// The page arguments of the paged calls. Slots and positions of a request stay
+// well inside a 32-bit int; element offsets are 64-bit.
+constexpr int kMaxPage = 4096;
+int check_pages(int P, int W, int page) {
+  if (page < 16 || page > kMaxPage || page % 16 != 0 || P < 1 || W < 1 || P > kMaxN / page ||
+      W > kMaxN / page)
+    return FA_B200_ERR_PAGES;
   return FA_B200_OK;
 }
 
@@ -833,6 +844,133 @@ int fa_b200_merge_partial(float* o, fa_b200_strides so, float* lse, fa_b200_stri
   return fab::launch_status("merge_partial_kernel");
 }
 
+size_t fa_b200_paged_table_workspace_bytes(int B) {
+  return B < 1 ? 0 : sizeof(fab::TableHead) + static_cast<size_t>(B) * sizeof(fab::TableRow);
+}
+
+int fa_b200_paged_extend(const int* new_lens, const int* lens, int* block_table,
+                         int64_t table_stride, const int* free_pages, const int* free_count,
+                         int* slots, int* granted, int* lens_out, int* free_count_out,
+                         void* workspace, size_t workspace_bytes, int B, int W, int P,
+                         int page_size, int T, void* stream) {
+  if (!new_lens || !lens || !block_table || !free_pages || !free_count || (!slots && T > 0) ||
+      !granted || !lens_out || !free_count_out)
+    return FA_B200_ERR_NULL_POINTER;
+  if (B < 1 || T < 0 || table_stride < W) return FA_B200_ERR_SHAPE;
+  if (int st = fab::check_pages(P, W, page_size)) return st;
+  if (!workspace || workspace_bytes < fa_b200_paged_table_workspace_bytes(B))
+    return FA_B200_ERR_WORKSPACE;
+  if (!fab::aligned16(workspace)) return FA_B200_ERR_ALIGNMENT;
+  int dev = 0, sms = 0;
+  int* err = nullptr;
+  if (int st = fab::device_setup(&dev, &err, &sms)) return st;
+  auto* head = static_cast<fab::TableHead*>(workspace);
+  const fab::ExtendArgs a{new_lens, lens, free_pages, free_count, block_table, slots, granted,
+                          lens_out, free_count_out, table_stride, head,
+                          reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size, T};
+  fab::extend_kernel<<<1, fab::kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return fab::launch_status("extend_kernel");
+}
+
+int fa_b200_paged_release(const unsigned char* finished, const int* lens, const int* block_table,
+                          int64_t table_stride, int* free_pages, const int* free_count,
+                          int* lens_out, int* free_count_out, void* workspace,
+                          size_t workspace_bytes, int B, int W, int P, int page_size,
+                          void* stream) {
+  if (!finished || !lens || !block_table || !free_pages || !free_count || !lens_out ||
+      !free_count_out)
+    return FA_B200_ERR_NULL_POINTER;
+  if (B < 1 || table_stride < W) return FA_B200_ERR_SHAPE;
+  if (int st = fab::check_pages(P, W, page_size)) return st;
+  if (!workspace || workspace_bytes < fa_b200_paged_table_workspace_bytes(B))
+    return FA_B200_ERR_WORKSPACE;
+  if (!fab::aligned16(workspace)) return FA_B200_ERR_ALIGNMENT;
+  int dev = 0, sms = 0;
+  int* err = nullptr;
+  if (int st = fab::device_setup(&dev, &err, &sms)) return st;
+  auto* head = static_cast<fab::TableHead*>(workspace);
+  const fab::ReleaseArgs a{finished, lens, block_table, free_count, free_pages, lens_out,
+                           free_count_out, table_stride, head,
+                           reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size};
+  fab::release_kernel<<<1, fab::kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  return fab::launch_status("release_kernel");
+}
+
+int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b200_strides sv,
+                         const int* slots, void* k_cache, fa_b200_strides skc, void* v_cache,
+                         fa_b200_strides svc, int T, int Hkv, int D, int P, int page_size,
+                         int dtype, void* stream) {
+  using fab::from_abi;
+  if (T < 0) return FA_B200_ERR_SHAPE;
+  if (!k_cache || !v_cache || (T > 0 && (!k || !v || !slots))) return FA_B200_ERR_NULL_POINTER;
+  if (D != 64 && D != 128) return FA_B200_ERR_HEAD_DIM;
+  if (Hkv < 1) return FA_B200_ERR_SHAPE;
+  if (int st = fab::check_pages(P, 1, page_size)) return st;
+  if (dtype != FA_B200_DTYPE_FP16 && dtype != FA_B200_DTYPE_BF16) return FA_B200_ERR_DTYPE;
+  const fab::AppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
+                          static_cast<uint16_t*>(k_cache), static_cast<uint16_t*>(v_cache),
+                          from_abi(sk), from_abi(sv), from_abi(skc), from_abi(svc), slots, T, Hkv,
+                          P, page_size};
+  if (!fab::aligned16(k) || !fab::aligned16(v) || !fab::aligned16(k_cache) ||
+      !fab::aligned16(v_cache) || !fab::strides_ok(a.sk, 2) || !fab::strides_ok(a.sv, 2) ||
+      !fab::strides_ok(a.skc, 2) || !fab::strides_ok(a.svc, 2))
+    return FA_B200_ERR_ALIGNMENT;
+  const long long blocks = (static_cast<long long>(T) * Hkv * (D / 8) + 255) / 256;
+  if (blocks > 0x7fffffffll) return FA_B200_ERR_TOO_LARGE;
+  if (T == 0) return FA_B200_OK;
+  int dev = 0;
+  int* err = nullptr;
+  if (int st = fab::device_setup(&dev, &err)) return st;
+  auto s = static_cast<cudaStream_t>(stream);
+  if (D == 64)
+    fab::append_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+  else
+    fab::append_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
+  return fab::launch_status("append_kernel");
+}
+
+size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size) {
+  (void)B, (void)Hq, (void)Hkv, (void)W, (void)D, (void)page_size;
+  return 0;
+}
+
+int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, fa_b200_strides skc,
+                       const void* v_cache, fa_b200_strides svc, const int* block_table,
+                       int64_t table_stride, const int* lens, void* o, fa_b200_strides so,
+                       float* lse, void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv,
+                       int D, int P, int W, int page_size, int dtype, void* stream) {
+  using fab::from_abi;
+  if (!q || !k_cache || !v_cache || !block_table || !lens || !o || !lse)
+    return FA_B200_ERR_NULL_POINTER;
+  if (int st = fab::check_shape(B, Hq, Hkv, 1, D)) return st;
+  if (table_stride < W) return FA_B200_ERR_SHAPE;
+  if (int st = fab::check_pages(P, W, page_size)) return st;
+  if (dtype != FA_B200_DTYPE_FP16 && dtype != FA_B200_DTYPE_BF16) return FA_B200_ERR_DTYPE;
+  fab::PagedAttnArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache),
+                       static_cast<const uint16_t*>(v_cache), static_cast<uint16_t*>(o), lse,
+                       from_abi(sq), from_abi(so), from_abi(skc), from_abi(svc), block_table, lens,
+                       table_stride, Hq, Hkv, P, W, page_size,
+                       1.4426950408889634f / sqrtf(static_cast<float>(D)), nullptr};
+  if (!fab::aligned16(q) || !fab::aligned16(k_cache) || !fab::aligned16(v_cache) ||
+      !fab::aligned16(o) || !fab::strides_ok(a.sq, 2) || !fab::strides_ok(a.so, 2) ||
+      !fab::strides_ok(a.skc, 2) || !fab::strides_ok(a.svc, 2))
+    return FA_B200_ERR_ALIGNMENT;
+  if (static_cast<long long>(B) * Hq > 0x7fffffffll) return FA_B200_ERR_TOO_LARGE;
+  if (workspace_bytes < fa_b200_paged_attn_workspace_bytes(B, Hq, Hkv, W, D, page_size))
+    return FA_B200_ERR_WORKSPACE;
+  (void)workspace;
+  int dev = 0;
+  if (int st = fab::device_setup(&dev, &a.err)) return st;
+  const unsigned blocks = static_cast<unsigned>(B) * Hq;
+  auto s = static_cast<cudaStream_t>(stream);
+  const bool bf = dtype == FA_B200_DTYPE_BF16;
+  if (D == 64 && bf) fab::paged_attn_kernel<64, true><<<blocks, 128, 0, s>>>(a);
+  if (D == 64 && !bf) fab::paged_attn_kernel<64, false><<<blocks, 128, 0, s>>>(a);
+  if (D == 128 && bf) fab::paged_attn_kernel<128, true><<<blocks, 128, 0, s>>>(a);
+  if (D == 128 && !bf) fab::paged_attn_kernel<128, false><<<blocks, 128, 0, s>>>(a);
+  return fab::launch_status("paged_attn_kernel");
+}
+
 size_t fa_b200_backward_workspace_bytes(int B, int Hq, int N) {
   if (B < 1 || Hq < 1 || N < 1 || N > fab::kMaxN) return 0;
   // Dv and LSE*log2e for every query row, each head padded to a multiple of
@@ -991,6 +1129,7 @@ const char* fa_b200_status_string(int status) {
     case FA_B200_ERR_DEVICE: return "current device is not an sm_100 (B200-class) GPU";
     case FA_B200_ERR_TOO_LARGE: return "problem exceeds a CUDA grid limit";
     case FA_B200_ERR_SCRATCH_LIMIT: return "problem exceeds the built-in scratch of the no-allocation backward";
+    case FA_B200_ERR_PAGES: return "page size must be a multiple of 16 up to 4096, and the pool and a table row hold 1 to 2^30 tokens";
     case FA_B200_ERR_UNCHECKED_BUILD: return "not a checked build (build with FA_B200_DEBUG=1 for the TMA checks)";
     default: return "unknown status";
   }

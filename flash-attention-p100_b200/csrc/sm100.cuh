@@ -45,6 +45,7 @@ enum DevErr : int {
   kErrTimeoutEpilogue = 4,
   kErrSmemAlign = 5,     // dynamic shared memory did not start 1024-byte aligned
   kErrSelftest = 6,      // the failure-detection self-test's deliberate timeout
+  kErrPage = 7,          // a block table entry names no page of the cache
 };
 
 // Kernels that need every byte of shared memory do not pad for alignment:

@@ -39,6 +39,9 @@ _DEVERR = {1: "a TMA producer waited too long for a free slot",
 
 
 def _device_error_message(code):
+    if code == 7:
+        return ("a block table named a page outside its cache (device error 7); its tokens were left "
+                "out of that attention")
     return (f"an attention kernel gave up a bounded internal wait (device error {code}: "
             f"{_DEVERR.get(code, 'unknown')}); the outputs of that call are incomplete")
 

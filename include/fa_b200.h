@@ -40,7 +40,9 @@ enum {
   FA_B200_ERR_TOO_LARGE = 9,       /* a grid dimension would exceed CUDA limits */
   FA_B200_ERR_SCRATCH_LIMIT = 10,  /* B*Hq*roundup(N,128) above fa_b200_backward_noalloc_max_rows() */
   FA_B200_ERR_DTYPE = 11,          /* dtype is not one of FA_B200_DTYPE_* */
-  FA_B200_ERR_UNCHECKED_BUILD = 12 /* fa_b200_debug_tma_check on a release build */
+  FA_B200_ERR_UNCHECKED_BUILD = 12, /* fa_b200_debug_tma_check on a release build */
+  FA_B200_ERR_PAGES = 13           /* page size not a multiple of 16 or above 4096, no pages, or
+                                    * P * page_size or W * page_size above 2^30 */
 };
 
 /* Element type of the 16-bit tensors (q, k, v, o, dO, dk, dv, a 16-bit dq) of
@@ -135,6 +137,79 @@ int fa_b200_merge_partial(float* o, fa_b200_strides so, float* lse, fa_b200_stri
                           fa_b200_strides slp, int B, int H, int N, int D, int dtype,
                           void* stream);
 
+/* ---- Paged key-value cache (no counterpart in the reference, which has no
+ * cache) ----
+ * k_cache and v_cache are (P, Hkv, page_size, D): P pages of page_size tokens,
+ * 16-bit, any strides with D contiguous (fa_b200_strides with batch = page,
+ * head, row = token), so pages stored token by token are read in place. The
+ * page size is a multiple of 16, at most 4096. A block table is int32 (B, W),
+ * its columns contiguous and its rows table_stride entries apart: row r lists
+ * request r's pages in order. lens is int32 (B), the tokens each request has.
+ * A token's slot is page * page_size + offset in its page. The free pages are
+ * the first *free_count entries of the stack free_pages (int32, P entries);
+ * they are taken from its top. All these live on the device and the calls read
+ * nothing back; the kernels check every length, page and slot against the
+ * pool. int32 pointers need 4-byte alignment only. */
+
+/* Bytes of device workspace for fa_b200_paged_extend and fa_b200_paged_release
+ * of B requests. */
+size_t fa_b200_paged_table_workspace_bytes(int B);
+
+/* Gives every request r room for n = max(new_lens[r], 0) more tokens. Requests
+ * are served in order: one is refused if lens[r] is negative, if lens[r] + n
+ * exceeds W * page_size, if its tokens end behind T in the call's packed
+ * tokens, or if it needs pages and the free ones do not cover its need and that
+ * of the requests before it (those too long for their row or for T apart). Writes
+ *   granted[r]     n, or 0 for a refused request
+ *   lens_out[r]    lens[r] + granted[r]
+ *   block_table    the new pages of the served requests, behind their pages so far
+ *   free_count_out the free pages left; the stack itself is not changed
+ *   slots[t], t < T  the packed tokens, request by request (refused ones too):
+ *                  their slots, -1 for a refused request's, behind the last
+ *                  token, and in an existing page whose id is not in [0, P)
+ * lens_out may be lens and free_count_out free_count. */
+int fa_b200_paged_extend(const int* new_lens, const int* lens, int* block_table,
+                         int64_t table_stride, const int* free_pages, const int* free_count,
+                         int* slots, int* granted, int* lens_out, int* free_count_out,
+                         void* workspace, size_t workspace_bytes, int B, int W, int P,
+                         int page_size, int T, void* stream);
+
+/* Takes the pages of every request with finished[r] != 0 back: its first
+ * ceil(lens[r] / page_size) table entries go onto the stack (requests in order,
+ * each one's pages in order), its length becomes 0. The block table is not
+ * changed. A page must be in one row only; pages beyond the stack's P entries
+ * are dropped. lens_out may be lens and free_count_out free_count. */
+int fa_b200_paged_release(const unsigned char* finished, const int* lens, const int* block_table,
+                          int64_t table_stride, int* free_pages, const int* free_count,
+                          int* lens_out, int* free_count_out, void* workspace,
+                          size_t workspace_bytes, int B, int W, int P, int page_size, void* stream);
+
+/* Writes T tokens' keys and values into their slots: k_cache[slot] = k[t],
+ * v_cache[slot] = v[t]. k and v are (T, Hkv, D) with D contiguous
+ * (fa_b200_strides head and row; batch is not used). Tokens whose slot is not in
+ * [0, P * page_size) are skipped; the others' slots must differ from each other. */
+int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b200_strides sv,
+                         const int* slots, void* k_cache, fa_b200_strides skc, void* v_cache,
+                         fa_b200_strides svc, int T, int Hkv, int D, int P, int page_size,
+                         int dtype, void* stream);
+
+/* Bytes of device workspace for fa_b200_paged_attn (0: none needed). */
+size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size);
+
+/* Attention of one token per request over its cached tokens 0 .. lens[r] - 1
+ * (the token itself among them, once it is appended): o (B, Hq, D) and lse
+ * (B, Hq) fp32 as fa_b200_forward gives them; q and o are (B, Hq, D)
+ * (fa_b200_strides batch and head; row is not used). A length below 0 counts as
+ * 0, one above W * page_size as W * page_size; a row of length 0 gets o = 0 and
+ * lse = -inf. What lies behind a request's last token is never used. A table
+ * entry outside [0, P) sets FA_B200_DEVERR_PAGE and its tokens are left out. The
+ * result does not depend on timing: equal inputs give equal bits. */
+int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, fa_b200_strides skc,
+                       const void* v_cache, fa_b200_strides svc, const int* block_table,
+                       int64_t table_stride, const int* lens, void* o, fa_b200_strides so,
+                       float* lse, void* workspace, size_t workspace_bytes, int B, int Hq, int Hkv,
+                       int D, int P, int W, int page_size, int dtype, void* stream);
+
 /* Stages of the backward, for fa_b200_backward_stages. */
 enum {
   FA_B200_STAGE_ROWSUM = 1,  /* Dv = rowsum(dO o O) into the workspace; also zeroes an
@@ -223,7 +298,9 @@ enum {
   FA_B200_DEVERR_TIMEOUT_COMPUTE = 3,   /* softmax / gradient warps waited too long for an MMA */
   FA_B200_DEVERR_TIMEOUT_EPILOGUE = 4,  /* an epilogue / read-out waited too long */
   FA_B200_DEVERR_SMEM_ALIGN = 5,        /* dynamic shared memory not 1024-byte aligned */
-  FA_B200_DEVERR_SELFTEST = 6           /* fa_b200_selftest_wait's deliberate timeout */
+  FA_B200_DEVERR_SELFTEST = 6,          /* fa_b200_selftest_wait's deliberate timeout */
+  FA_B200_DEVERR_PAGE = 7               /* fa_b200_paged_attn met a block table entry that names
+                                         * no page of the cache; its keys were left out */
 };
 
 /* Reads the device error word the kernels set when a bounded internal wait

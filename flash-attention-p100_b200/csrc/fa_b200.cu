@@ -94,6 +94,10 @@ void set_smem_all() {
   set_smem(bwd_dq_kernel<128, BF>, DqCfg<128>::SMEM);
   set_smem(bwd_fused_kernel<64, BF>, FusedCfg<64>::SMEM);
   set_smem(bwd_fused_kernel<128, BF>, FusedCfg<128>::SMEM);
+  set_smem(paged_attn_kernel<64, BF, 1>, PagedCfg<64>::SMEM);
+  set_smem(paged_attn_kernel<64, BF, 2>, PagedCfg<64>::SMEM);
+  set_smem(paged_attn_kernel<128, BF, 1>, PagedCfg<128>::SMEM);
+  set_smem(paged_attn_kernel<128, BF, 2>, PagedCfg<128>::SMEM);
 }
 
 // One-time, per-device set-up with that device current: architecture check,
@@ -213,6 +217,41 @@ int launch_status(const char* kernel) {
   if (e == cudaSuccess) return FA_B200_OK;
   set_last_error("launch of %s failed: %s", kernel, cudaGetErrorString(e));
   return FA_B200_ERR_LAUNCH;
+}
+
+// Workspace of the paged attention: per block of the launch the unit it began
+// and two partial results of a row tile's heads.
+size_t paged_workspace(int group, int D) {
+  const size_t rows = 2 * static_cast<size_t>(std::min(group, 32)) * kPagedMaxBlocks;
+  return kPagedMaxBlocks * sizeof(int4) + rows * (sizeof(float2) + D * sizeof(float));
+}
+
+template <int D, bool BF, int MT>
+int paged_attn_launch(PagedAttnArgs& a, int sms, cudaStream_t stream) {
+  using C = PagedCfg<D>;
+  const int group = a.Hq / a.Hkv;
+  a.row_tiles = (group + 16 * MT - 1) / (16 * MT);
+  // two blocks an SM, fewer where the table has no room for so many steps
+  const double most = static_cast<double>(a.B) * a.Hkv * a.row_tiles *
+                      ((a.W * a.page + C::STEP - 1) / C::STEP);
+  const int blocks = static_cast<int>(std::min<double>(std::min(2 * sms, kPagedMaxBlocks), most));
+  paged_attn_kernel<D, BF, MT><<<blocks, 128, C::SMEM, stream>>>(a);
+  if (int st = launch_status("paged_attn_kernel")) return st;
+  paged_join_kernel<D, BF><<<dim3(blocks, std::min(group, 8)), 128, 0, stream>>>(a, 16 * MT);
+  return launch_status("paged_join_kernel");
+}
+
+template <int D, bool BF>
+int paged_attn_impl(PagedAttnArgs& a, void* workspace, void* stream) {
+  int dev = 0, sms = 0;
+  if (int st = device_setup(&dev, &a.err, &sms)) return st;
+  const size_t rows = 2 * static_cast<size_t>(std::min(a.Hq / a.Hkv, 32)) * kPagedMaxBlocks;
+  a.split = static_cast<int4*>(workspace);
+  a.part_o = reinterpret_cast<float*>(a.split + kPagedMaxBlocks);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
+  auto s = static_cast<cudaStream_t>(stream);
+  return a.Hq / a.Hkv <= 16 ? paged_attn_launch<D, BF, 1>(a, sms, s)
+                            : paged_attn_launch<D, BF, 2>(a, sms, s);
 }
 
 // An fp32 dQ is produced by the fused kernel: one pass, dQ added into the
@@ -930,8 +969,8 @@ int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b2
 }
 
 size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size) {
-  (void)B, (void)Hq, (void)Hkv, (void)W, (void)D, (void)page_size;
-  return 0;
+  if (fab::check_shape(B, Hq, Hkv, 1, D) || fab::check_pages(1, W, page_size)) return 0;
+  return fab::paged_workspace(Hq / Hkv, D);
 }
 
 int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, fa_b200_strides skc,
@@ -946,29 +985,27 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
   if (table_stride < W) return FA_B200_ERR_SHAPE;
   if (int st = fab::check_pages(P, W, page_size)) return st;
   if (dtype != FA_B200_DTYPE_FP16 && dtype != FA_B200_DTYPE_BF16) return FA_B200_ERR_DTYPE;
-  fab::PagedAttnArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_cache),
-                       static_cast<const uint16_t*>(v_cache), static_cast<uint16_t*>(o), lse,
-                       from_abi(sq), from_abi(so), from_abi(skc), from_abi(svc), block_table, lens,
-                       table_stride, Hq, Hkv, P, W, page_size,
-                       1.4426950408889634f / sqrtf(static_cast<float>(D)), nullptr};
+  if (!workspace || workspace_bytes < fab::paged_workspace(Hq / Hkv, D)) return FA_B200_ERR_WORKSPACE;
+  fab::PagedAttnArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.k_cache = static_cast<const uint16_t*>(k_cache);
+  a.v_cache = static_cast<const uint16_t*>(v_cache);
+  a.o = static_cast<uint16_t*>(o);
+  a.lse = lse;
+  a.sq = from_abi(sq), a.so = from_abi(so), a.skc = from_abi(skc), a.svc = from_abi(svc);
+  a.table = block_table, a.lens = lens, a.table_stride = table_stride;
+  a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.P = P, a.W = W, a.page = page_size;
+  a.scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
   if (!fab::aligned16(q) || !fab::aligned16(k_cache) || !fab::aligned16(v_cache) ||
-      !fab::aligned16(o) || !fab::strides_ok(a.sq, 2) || !fab::strides_ok(a.so, 2) ||
-      !fab::strides_ok(a.skc, 2) || !fab::strides_ok(a.svc, 2))
+      !fab::aligned16(o) || !fab::aligned16(workspace) || !fab::strides_ok(a.sq, 2) ||
+      !fab::strides_ok(a.so, 2) || !fab::strides_ok(a.skc, 2) || !fab::strides_ok(a.svc, 2))
     return FA_B200_ERR_ALIGNMENT;
-  if (static_cast<long long>(B) * Hq > 0x7fffffffll) return FA_B200_ERR_TOO_LARGE;
-  if (workspace_bytes < fa_b200_paged_attn_workspace_bytes(B, Hq, Hkv, W, D, page_size))
-    return FA_B200_ERR_WORKSPACE;
-  (void)workspace;
-  int dev = 0;
-  if (int st = fab::device_setup(&dev, &a.err)) return st;
-  const unsigned blocks = static_cast<unsigned>(B) * Hq;
-  auto s = static_cast<cudaStream_t>(stream);
   const bool bf = dtype == FA_B200_DTYPE_BF16;
-  if (D == 64 && bf) fab::paged_attn_kernel<64, true><<<blocks, 128, 0, s>>>(a);
-  if (D == 64 && !bf) fab::paged_attn_kernel<64, false><<<blocks, 128, 0, s>>>(a);
-  if (D == 128 && bf) fab::paged_attn_kernel<128, true><<<blocks, 128, 0, s>>>(a);
-  if (D == 128 && !bf) fab::paged_attn_kernel<128, false><<<blocks, 128, 0, s>>>(a);
-  return fab::launch_status("paged_attn_kernel");
+  if (D == 64)
+    return bf ? fab::paged_attn_impl<64, true>(a, workspace, stream)
+              : fab::paged_attn_impl<64, false>(a, workspace, stream);
+  return bf ? fab::paged_attn_impl<128, true>(a, workspace, stream)
+            : fab::paged_attn_impl<128, false>(a, workspace, stream);
 }
 
 size_t fa_b200_backward_workspace_bytes(int B, int Hq, int N) {

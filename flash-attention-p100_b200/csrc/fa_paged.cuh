@@ -266,6 +266,25 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // ---------------------------------------------------------------------------
 // attention of one new token per request
 // ---------------------------------------------------------------------------
+// o_h = sum_j softmax_j(q_h . k_j / sqrt(D)) v_j over a request's cached tokens.
+// Every cached byte is read once for Hq/Hkv query heads: 1 FLOP per byte and
+// head, so HBM is the bound, and the matrix instruction only has to keep up
+// with the loads. That is why this is mma.sync and not tcgen05: a group of 1 to
+// 16 heads fills one m16 fragment (a tcgen05 tile would be 128 rows), operands
+// come straight out of the loaded tile, and no accumulator leaves registers.
+//
+// Work is cut along the keys, not along requests: all (request, kv head, row
+// tile) units in order, each as steps of STEP keys, form one line of steps that
+// is divided evenly over the blocks of the launch. A block walks its stretch
+// through unit after unit; a unit that lies within one stretch is finished
+// there, one cut by a border is left as partial results (o, max, sum in fp32)
+// that paged_join_kernel adds up in the order of the keys. So one long request
+// and a thousand ragged ones both keep every SM loading, and the result does not
+// depend on timing.
+//
+// Inside a block each warp takes KEYS of a step's keys into a ring of its own
+// (cp.async, 16 bytes a lane), three steps deep, across unit borders too: the
+// loads never drain, and warps meet only where a unit ends.
 struct PagedAttnArgs {
   const uint16_t *q, *k_cache, *v_cache;
   uint16_t* o;
@@ -273,81 +292,508 @@ struct PagedAttnArgs {
   Strides sq, so, skc, svc;  // q, o: b request, h head; caches: b page, h head, n token
   const int *table, *lens;
   long long table_stride;
-  int Hq, Hkv, P, W, page;
-  float scale;  // log2(e) / sqrt(D)
+  int B, Hq, Hkv, P, W, page;
+  int row_tiles;   // row tiles of 16 * MT heads in a group
+  float scale;     // log2(e) / sqrt(D)
+  int4* split;     // per block: the unit whose first part it holds (b, unit in b, last block), x < 0: none
+  float2* part_ml; // per block two partial results: [2 block + first][row] max and sum
+  float* part_o;   // ... and [2 block + first][row][D]
   int* err;
 };
 
+template <int D>
+struct PagedCfg {
+  static constexpr int WARPS = 4;
+  static constexpr int STAGES = 3;
+  static constexpr int KEYS = 2048 / D;       // of a warp in a step: 4 KB of K, 4 KB of V
+  static constexpr int STEP = WARPS * KEYS;
+  static constexpr int GROUPS = KEYS / 16;    // runs of 16 keys: each lies in one page
+  static constexpr int TILE = KEYS * D * 2;   // bytes of a warp's K (or V) of a step
+  static constexpr int RING = WARPS * STAGES * 2 * TILE;
+  static constexpr int MERGE = 16 * D * 4;    // one warp's fp32 result of 16 rows
+  static constexpr int SMEM = RING + 2 * MERGE;
+};
+
+constexpr int kPagedMaxBlocks = 320;  // blocks of a launch at most: sizes the workspace
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// c (16 x 8 fp32) += a (16 x 16) b (16 x 8), 16-bit operands
+template <bool BF>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if (BF)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 template <bool BF>
 __device__ __forceinline__ float2 unpack16(uint32_t x) {
   if (BF) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 template <bool BF>
-__device__ __forceinline__ uint16_t round16(float x) {
-  if (BF) return __bfloat16_as_ushort(__float2bfloat16_rn(x));
-  return __half_as_ushort(__float2half_rn(x));
+__device__ __forceinline__ uint32_t pack16(float x, float y) {
+  if (BF) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One block per (request, query head); each warp takes every fourth key, each
-// lane D/32 of its columns.
-template <int D, bool BF>
+// A place on the line of steps.
+struct PagedAt {
+  int b, unit;  // request; kv head * row_tiles + row tile
+  int t, nt;    // step of the unit, steps of the unit
+  int len;
+};
+
+// MT m16 fragments of heads per block: 1 up to 16 heads a group, 2 above (a
+// group above 32 is cut into row tiles, each of which reads the cache again).
+template <int D, bool BF, int MT>
 __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) {
-  constexpr int C = D / 32;
-  const int b = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq, kh = h / (a.Hq / a.Hkv);
+  using C = PagedCfg<D>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ long long s_sum[C::WARPS];
+  __shared__ int s_b, s_valid[C::WARPS][C::STAGES];
+  __shared__ long long s_at;
+  __shared__ float2 s_ml[C::WARPS][16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int len = min(max(a.lens[b], 0), a.W * a.page);
-  float q[C], o[C] = {}, m = -INFINITY, l = 0.f;
-  for (int i = 0; i < C; i += 2) {
-    const float2 x = unpack16<BF>(*reinterpret_cast<const uint32_t*>(a.q + a.sq.at(b, h, 0) + lane * C + i));
-    q[i] = x.x;
-    q[i + 1] = x.y;
+  const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
+  const int cap = a.W * a.page;
+  const auto length = [&](int b) { return min(max(a.lens[b], 0), cap); };
+  const auto steps = [&](int len) { return (len + C::STEP - 1) / C::STEP; };
+
+  // ---- this block's stretch [g0, g1) of the line; every block adds up the lengths itself ----
+  long long total, g0, g1;
+  int blocks;
+  {
+    const int per = (a.B + 127) / 128;
+    const int b0 = min(static_cast<int>(threadIdx.x) * per, a.B), b1 = min(b0 + per, a.B);
+    long long mine = 0;
+    for (int b = b0; b < b1; ++b) mine += static_cast<long long>(steps(length(b))) * units;
+    long long sum = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += y;
+    }
+    if (lane == 31) s_sum[warp] = sum;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < C::WARPS; ++w) {
+      if (w < warp) sum += s_sum[w];
+      total += s_sum[w];
+    }
+    blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
+    const int c = blockIdx.x;
+    g0 = c < blocks ? c * total / blocks : total;
+    g1 = c < blocks ? (c + 1) * total / blocks : total;
+    long long at = sum - mine;
+    if (at <= g0 && g0 < sum) {
+      int b = b0;
+      for (;; ++b) {
+        const long long n = static_cast<long long>(steps(length(b))) * units;
+        if (g0 < at + n) break;
+        at += n;
+      }
+      s_b = b;
+      s_at = g0 - at;
+    }
   }
-  for (int j = warp; j < len; j += 4) {
-    const int id = a.table[b * a.table_stride + j / a.page];
-    if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.P)) {
-      if (lane == 0) atomicCAS(a.err, 0, static_cast<int>(kErrPage));
-      continue;
-    }
-    const uint16_t* k = a.k_cache + a.skc.at(id, kh, j % a.page) + lane * C;
-    const uint16_t* v = a.v_cache + a.svc.at(id, kh, j % a.page) + lane * C;
-    float s = 0.f;
-    for (int i = 0; i < C; i += 2) {
-      const float2 x = unpack16<BF>(*reinterpret_cast<const uint32_t*>(k + i));
-      s += q[i] * x.x + q[i + 1] * x.y;
-    }
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    s *= a.scale;
-    const float mn = fmaxf(m, s), ref = mn == -INFINITY ? 0.f : mn;
-    const float w = exp2f(m - ref), p = exp2f(s - ref);
-    m = mn;
-    l = l * w + p;
-    for (int i = 0; i < C; i += 2) {
-      const float2 x = unpack16<BF>(*reinterpret_cast<const uint32_t*>(v + i));
-      o[i] = o[i] * w + p * x.x;
-      o[i + 1] = o[i + 1] * w + p * x.y;
-    }
-  }
-  __shared__ float so[4][D], sm[4], sl[4];
-  for (int i = 0; i < C; ++i) so[warp][lane * C + i] = o[i];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
+  if (threadIdx.x == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  // rows without a token
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (length(b) != 0) continue;
+    for (int i = threadIdx.x; i < a.Hq * (D / 2); i += 128)
+      *reinterpret_cast<uint32_t*>(a.o + a.so.at(b, i / (D / 2), 0) + i % (D / 2) * 2) = 0;
+    for (int h = threadIdx.x; h < a.Hq; h += 128) a.lse[static_cast<long long>(b) * a.Hq + h] = -INFINITY;
   }
   __syncthreads();
-  const float top = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f, acc = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    const float e = exp2f(sm[w] - ref);
-    sum += sl[w] * e;
-    if (threadIdx.x < D) acc += so[w][threadIdx.x] * e;
+  if (g0 == g1) return;
+
+  PagedAt at;
+  at.b = s_b;
+  at.len = length(at.b);
+  at.nt = steps(at.len);
+  at.unit = static_cast<int>(s_at / at.nt);
+  at.t = static_cast<int>(s_at % at.nt);
+  const auto advance = [&](PagedAt& x) {
+    if (++x.t < x.nt) return;
+    x.t = 0;
+    if (++x.unit < units) return;
+    x.unit = 0;
+    do x.len = length(++x.b); while (x.len == 0);
+    x.nt = steps(x.len);
+  };
+
+  // ---- loads ----
+  const uint32_t ring = smem_u32(smem) + warp * C::STAGES * 2 * C::TILE;
+  constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows a warp covers at once
+  const int lc = lane % CH, lr = lane / CH;
+  int ids[C::GROUPS];
+  PagedAt ld = at;
+  const auto fetch_ids = [&]() {
+#pragma unroll
+    for (int g = 0; g < C::GROUPS; ++g) {
+      const int key = ld.t * C::STEP + warp * C::KEYS + g * 16;
+      ids[g] = key < ld.len ? a.table[ld.b * a.table_stride + key / a.page] : 0;
+    }
+  };
+  const auto issue = [&](int stage) {
+    const uint32_t kd = ring + stage * 2 * C::TILE + lr * (D * 2);
+    const int kv_head = ld.unit / a.row_tiles;
+    int valid = 0;
+#pragma unroll
+    for (int g = 0; g < C::GROUPS; ++g) {
+      const int key = ld.t * C::STEP + warp * C::KEYS + g * 16;
+      int n = min(max(ld.len - key, 0), 16);
+      int id = ids[g];
+      if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.P)) {
+        if (n && lane == 0) atomicCAS(a.err, 0, static_cast<int>(kErrPage));
+        n = id = 0;
+      }
+      valid |= n << (8 * g);
+      const int off = n ? key % a.page : 0;
+      const uint16_t* k = a.k_cache + a.skc.at(id, kv_head, off + lr) + lc * 8;
+      const uint16_t* v = a.v_cache + a.svc.at(id, kv_head, off + lr) + lc * 8;
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const int row = i * RPI + lr;           // of the 16
+        const int bytes = row < n ? 16 : 0;     // the rest is filled with zeros, not read
+        const uint32_t dst = kd + (g * 16 + i * RPI) * (D * 2) + ((lc ^ (row & 7)) << 4);
+        cp_async16(dst, k + i * RPI * a.skc.n, bytes);
+        cp_async16(dst + C::TILE, v + i * RPI * a.svc.n, bytes);
+      }
+    }
+    if (lane == 0) s_valid[warp][stage] = valid;
+  };
+  const long long n_steps = g1 - g0;
+  long long issued = 0;
+  fetch_ids();
+  const auto issue_next = [&](int stage) {
+    if (issued < n_steps) {
+      issue(stage);
+      if (++issued < n_steps) {
+        advance(ld);
+        fetch_ids();
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) issue_next(s);
+
+  // ---- per unit state ----
+  // Weights are 2^(s - m + kBias): m is the running maximum when it last grew by
+  // more than 2^8 (scaling o and l only then), and in fp16 the bias keeps weights
+  // down to 2^-21 of the largest out of the subnormals (at most 2^15).
+  constexpr float kBias = BF ? 0.f : 7.f;
+  uint32_t qf[MT][D / 16][4];
+  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  const auto begin_unit = [&]() {
+    const int rt = at.unit % a.row_tiles, head0 = at.unit / a.row_tiles * group;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = (rt * MT + mt) * 16 + e * 8 + lane / 4;
+        const uint16_t* q = a.q + a.sq.at(at.b, head0 + min(r, group - 1), 0) + (lane & 3) * 2;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          qf[mt][ks][e] = r < group ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
+          qf[mt][ks][e + 2] = r < group ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
+        }
+        m[mt][e] = -INFINITY;
+        l[mt][e] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][i][e] = 0.f;
+    }
+  };
+  // scales this thread's rows of fragment mt by w[0], w[1]
+  const auto scale_o = [&](int mt, float w0, float w1) {
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i) {
+      o[mt][i][0] *= w0;
+      o[mt][i][1] *= w0;
+      o[mt][i][2] *= w1;
+      o[mt][i][3] *= w1;
+    }
+  };
+
+  int first_t = at.t;
+  begin_unit();
+  int stage = C::STAGES - 1;
+  for (long long it = 0; it < n_steps; ++it) {
+    const int free_stage = stage;
+    stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+    cp_async_wait<C::STAGES - 2>();
+    __syncwarp();   // the step's rows are in, and every lane has left the stage before it
+    issue_next(free_stage);
+    const int valid = s_valid[warp][stage];
+    const uint32_t kt = ring + stage * 2 * C::TILE, vt = kt + C::TILE;
+#pragma unroll
+    for (int g = 0; g < C::GROUPS; ++g) {
+      const int n = (valid >> (8 * g)) & 255;
+      if (n == 0) continue;
+      float s[MT][2][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][0][e] = s[mt][1][e] = 0.f;
+      {
+        const int row = g * 16 + (lane >> 4) * 8 + (lane & 7);
+        const uint32_t base = kt + row * (D * 2);
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) {
+          uint32_t f[4];
+          ldsm4(f, base + (((ks * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<BF>(s[mt][0], qf[mt][ks], f[0], f[1]);
+            mma16<BF>(s[mt][1], qf[mt][ks], f[2], f[3]);
+          }
+        }
+      }
+      uint32_t p[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float& x = s[mt][h][e];
+            x = h * 8 + (lane & 3) * 2 + (e & 1) < n ? x * a.scale : -INFINITY;
+            top[e >> 1] = fmaxf(top[e >> 1], x);
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+        }
+        if (__any_sync(0xffffffffu, top[0] > m[mt][0] + 8.f || top[1] > m[mt][1] + 8.f)) {
+          float w[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float mn = fmaxf(m[mt][e], top[e]);
+            w[e] = mn == -INFINITY ? 1.f : exp2f(m[mt][e] - mn);
+            m[mt][e] = mn;
+            l[mt][e] *= w[e];
+          }
+          scale_o(mt, w[0], w[1]);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float ref = m[mt][e] == -INFINITY ? 0.f : m[mt][e] - kBias;
+            // the sum takes the weights as the product with v takes them: rounded
+            const uint32_t w = pack16<BF>(exp2f(s[mt][h][2 * e] - ref), exp2f(s[mt][h][2 * e + 1] - ref));
+            const float2 r = unpack16<BF>(w);
+            l[mt][e] += r.x + r.y;
+            p[mt][2 * h + e] = w;
+          }
+      }
+      {
+        const int row = g * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
+        const uint32_t base = vt + row * (D * 2);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) {
+          uint32_t f[4];
+          ldsm4_t(f, base + (((dt * 2 + (lane >> 4)) ^ (row & 7)) << 4));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<BF>(o[mt][2 * dt], p[mt], f[0], f[1]);
+            mma16<BF>(o[mt][2 * dt + 1], p[mt], f[2], f[3]);
+          }
+        }
+      }
+    }
+
+    // ---- end of the unit, or of the stretch: add up the warps ----
+    if (at.t + 1 < at.nt && it + 1 < n_steps) {
+      ++at.t;
+      continue;
+    }
+    const bool whole = first_t == 0 && at.t + 1 == at.nt;
+    const int rt = at.unit % a.row_tiles, head0 = at.unit / a.row_tiles * group;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
+        l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
+      }
+      float4* buf = reinterpret_cast<float4*>(smem + C::RING);
+      // warps 2 and 3 hand their rows to 0 and 1, then 1 to 0
+#pragma unroll
+      for (int half = C::WARPS / 2; half >= 1; half >>= 1) {
+        __syncthreads();   // the buffers and s_ml are free
+        if (warp >= half && warp < 2 * half) {
+          float4* mine = buf + (warp - half) * (C::MERGE / 16);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+            mine[i * 32 + lane] = make_float4(o[mt][i][0], o[mt][i][1], o[mt][i][2], o[mt][i][3]);
+          if ((lane & 3) == 0) {
+            s_ml[warp][lane / 4] = make_float2(m[mt][0], l[mt][0]);
+            s_ml[warp][lane / 4 + 8] = make_float2(m[mt][1], l[mt][1]);
+          }
+        }
+        __syncthreads();
+        if (warp < half) {
+          float w[2], wo[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 x = s_ml[warp + half][lane / 4 + 8 * e];
+            const float mn = fmaxf(m[mt][e], x.x);
+            w[e] = mn == -INFINITY ? 1.f : exp2f(m[mt][e] - mn);
+            wo[e] = mn == -INFINITY ? 1.f : exp2f(x.x - mn);
+            m[mt][e] = mn;
+            l[mt][e] = l[mt][e] * w[e] + x.y * wo[e];
+          }
+          const float4* other = buf + warp * (C::MERGE / 16);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            const float4 x = other[i * 32 + lane];
+            o[mt][i][0] = o[mt][i][0] * w[0] + x.x * wo[0];
+            o[mt][i][1] = o[mt][i][1] * w[0] + x.y * wo[0];
+            o[mt][i][2] = o[mt][i][2] * w[1] + x.z * wo[1];
+            o[mt][i][3] = o[mt][i][3] * w[1] + x.w * wo[1];
+          }
+        }
+      }
+      if (warp == 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int lr16 = mt * 16 + e * 8 + lane / 4, r = rt * MT * 16 + lr16;
+          if (r >= group) continue;
+          if (whole) {
+            const float inv = 1.f / l[mt][e];
+            uint16_t* out = a.o + a.so.at(at.b, head0 + r, 0) + (lane & 3) * 2;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+              *reinterpret_cast<uint32_t*>(out + i * 8) =
+                  pack16<BF>(o[mt][i][2 * e] * inv, o[mt][i][2 * e + 1] * inv);
+            if ((lane & 3) == 0)
+              a.lse[static_cast<long long>(at.b) * a.Hq + head0 + r] =
+                  0.6931471805599453f * (m[mt][e] - kBias + log2f(l[mt][e]));
+          } else {
+            const int rows = min(group, MT * 16);
+            const long long slot = (2ll * blockIdx.x + (first_t == 0)) * rows + lr16;
+            float* out = a.part_o + slot * D + (lane & 3) * 2;
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+              *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+            if ((lane & 3) == 0) a.part_ml[slot] = make_float2(m[mt][e], l[mt][e]);
+          }
+        }
+      }
+    }
+    if (!whole && first_t == 0 && threadIdx.x == 0) {
+      // the block that holds the unit's last step
+      const long long last = g1 - 1 + (at.nt - 1 - at.t);
+      a.split[blockIdx.x] = make_int4(at.b, at.unit, static_cast<int>(((last + 1) * blocks - 1) / total), 0);
+    }
+    if (it + 1 < n_steps) {
+      advance(at);
+      first_t = 0;
+      begin_unit();
+    }
   }
-  if (threadIdx.x < D)
-    a.o[a.so.at(b, h, 0) + threadIdx.x] = round16<BF>(len ? acc / sum : 0.f);
-  if (threadIdx.x == 0)
-    a.lse[static_cast<long long>(b) * a.Hq + h] =
-        len ? 0.6931471805599453f * (top + log2f(sum)) : -INFINITY;
+}
+
+// Adds the parts of the units that a border of paged_attn_kernel cut: block x
+// takes the unit whose first part block x of that launch holds, blocks y its
+// rows in turn. The parts are those of consecutive blocks, so in key order.
+template <int D, bool BF>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, int row_tile) {
+  constexpr int COLS = D / 4, PARTS = 128 / COLS;
+  constexpr float kBias = BF ? 0.f : 7.f;
+  __shared__ float2 s_ml[kPagedMaxBlocks];
+  __shared__ float4 s_o[128];
+  __shared__ float s_red[4];
+  const int4 unit = a.split[blockIdx.x];
+  if (unit.x < 0) return;
+  const int group = a.Hq / a.Hkv, rt = unit.y % a.row_tiles, head0 = unit.y / a.row_tiles * group;
+  const int rows = min(group, row_tile), n = unit.z - static_cast<int>(blockIdx.x) + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int col = threadIdx.x % COLS, part = threadIdx.x / COLS;
+  // part i is the second partial result of the first block, the first one of the others
+  const auto slot = [&](int i, int r) {
+    return (2ll * (blockIdx.x + i) + (i == 0)) * rows + r;
+  };
+  for (int r = blockIdx.y; r < rows && rt * row_tile + r < group; r += gridDim.y) {
+    __syncthreads();
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < n; i += 128) {
+      const float2 x = a.part_ml[slot(i, r)];
+      s_ml[i] = x;
+      top = fmaxf(top, x.x);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    if (lane == 0) s_red[warp] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = part; i < n; i += PARTS) {
+      const float4 x = *reinterpret_cast<const float4*>(a.part_o + slot(i, r) * D + col * 4);
+      const float w = exp2f(s_ml[i].x - ref);
+      sum += s_ml[i].y * w;
+      acc.x += x.x * w;
+      acc.y += x.y * w;
+      acc.z += x.z * w;
+      acc.w += x.w * w;
+    }
+    s_o[threadIdx.x] = acc;
+    __syncthreads();
+    if (col == 0) s_ml[part].y = sum;   // s_ml is read
+    __syncthreads();
+    if (part == 0) {
+      sum = s_ml[0].y;
+#pragma unroll
+      for (int i = 1; i < PARTS; ++i) {
+        const float4 x = s_o[i * COLS + col];
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+        sum += s_ml[i].y;
+      }
+      const float inv = 1.f / sum;
+      const int head = head0 + rt * row_tile + r;
+      *reinterpret_cast<uint2*>(a.o + a.so.at(unit.x, head, 0) + col * 4) =
+          make_uint2(pack16<BF>(acc.x * inv, acc.y * inv), pack16<BF>(acc.z * inv, acc.w * inv));
+      if (col == 0)
+        a.lse[static_cast<long long>(unit.x) * a.Hq + head] = 0.6931471805599453f * (top - kBias + log2f(sum));
+    }
+  }
 }
 
 }  // namespace fab

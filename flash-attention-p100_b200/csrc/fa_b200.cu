@@ -219,6 +219,29 @@ int launch_status(const char* kernel) {
   return FA_B200_ERR_LAUNCH;
 }
 
+// Launches a kernel that waits (griddepcontrol.wait) for the launch before it on
+// `stream`: its blocks are scheduled while that one's last blocks still run.
+template <typename... Params, typename... Args>
+int launch_after(void (*kernel)(Params...), const char* name, dim3 grid, int threads,
+                 cudaStream_t stream, const Args&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  return launch_status(name);
+}
+
+// Threads of a one-block launch with `work` independent items.
+int table_threads(long long work) {
+  return static_cast<int>(std::min<long long>(kTableThreads, std::max<long long>(128, (work + 31) / 32 * 32)));
+}
+
 // Workspace of the paged attention: per block of the launch the unit it began
 // and two partial results of a row tile's heads.
 size_t paged_workspace(int group, int D) {
@@ -237,8 +260,8 @@ int paged_attn_launch(PagedAttnArgs& a, int sms, cudaStream_t stream) {
   const int blocks = static_cast<int>(std::min<double>(std::min(2 * sms, kPagedMaxBlocks), most));
   paged_attn_kernel<D, BF, MT><<<blocks, 128, C::SMEM, stream>>>(a);
   if (int st = launch_status("paged_attn_kernel")) return st;
-  paged_join_kernel<D, BF><<<dim3(blocks, std::min(group, 8)), 128, 0, stream>>>(a, 16 * MT);
-  return launch_status("paged_join_kernel");
+  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel", dim3(blocks, std::min(group, 8)),
+                      128, stream, a, 16 * MT);
 }
 
 template <int D, bool BF>
@@ -907,8 +930,15 @@ int fa_b200_paged_extend(const int* new_lens, const int* lens, int* block_table,
   const fab::ExtendArgs a{new_lens, lens, free_pages, free_count, block_table, slots, granted,
                           lens_out, free_count_out, table_stride, head,
                           reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size, T};
-  fab::extend_kernel<<<1, fab::kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  return fab::launch_status("extend_kernel");
+  auto s = static_cast<cudaStream_t>(stream);
+  const bool wide = T > fab::kTableWide;
+  fab::extend_kernel<<<1, fab::table_threads(std::max(B, T / fab::kSlotRun)), 0, s>>>(a, !wide);
+  if (int st = fab::launch_status("extend_kernel")) return st;
+  if (!wide) return FA_B200_OK;
+  const long long runs = (T + fab::kSlotRun - 1ll) / fab::kSlotRun;
+  return fab::launch_after(fab::extend_fill_kernel, "extend_fill_kernel",
+                           dim3(static_cast<unsigned>(std::min<long long>((runs + 255) / 256, 8 * sms))),
+                           256, s, a);
 }
 
 int fa_b200_paged_release(const unsigned char* finished, const int* lens, const int* block_table,
@@ -931,8 +961,15 @@ int fa_b200_paged_release(const unsigned char* finished, const int* lens, const 
   const fab::ReleaseArgs a{finished, lens, block_table, free_count, free_pages, lens_out,
                            free_count_out, table_stride, head,
                            reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size};
-  fab::release_kernel<<<1, fab::kTableThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  return fab::launch_status("release_kernel");
+  auto s = static_cast<cudaStream_t>(stream);
+  const long long runs = static_cast<long long>(B) * ((W + fab::kReleaseRun - 1) / fab::kReleaseRun);
+  const bool wide = std::min<long long>(P, static_cast<long long>(B) * W) > fab::kTableWide;
+  fab::release_kernel<<<1, fab::table_threads(std::max<long long>(B, wide ? 0 : 32 * runs)), 0, s>>>(a, !wide);
+  if (int st = fab::launch_status("release_kernel")) return st;
+  if (!wide) return FA_B200_OK;
+  return fab::launch_after(fab::release_fill_kernel, "release_fill_kernel",
+                           dim3(static_cast<unsigned>(std::min<long long>((runs + 7) / 8, 8 * sms))), 256,
+                           s, a);
 }
 
 int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b200_strides sv,

@@ -19,9 +19,20 @@ namespace fab {
 // ---------------------------------------------------------------------------
 // block tables
 // ---------------------------------------------------------------------------
+// Both calls are two running sums over the requests, by one block, and then
+// writes that need only their results. The sums are latency: a load, two scans,
+// a store. The writes go by the same block where the host knows that they are
+// few, else by a second launch that fills the GPU and whose start overlaps the
+// first (kTableWide).
 constexpr int kTableThreads = 1024;
+// Slots (extend) or table entries (release) above which the second launch pays:
+// one block writes about 2 a nanosecond, a launch more costs about 1.5 us.
+constexpr int kTableWide = 8192;
+// Up to this many tokens a request's own thread writes them (a decoding step);
+// a page holds 16 or more, so they take at most one new page.
+constexpr int kSlotsByRow = 4;
 
-// What the second half of extend and release needs of a request.
+// What the writes need of a request.
 struct alignas(16) TableRow {
   int tok;    // first token of the request in the call's packed tokens (extend)
   int page;   // first page of the request in the call's pages
@@ -29,15 +40,22 @@ struct alignas(16) TableRow {
   int count;  // tokens granted (extend) or pages given back (release)
 };
 struct alignas(16) TableHead {
-  int pages;  // pages the call takes or gives back
-  int free;   // free pages before the call
-  int pad[2];
+  int pages;    // pages the call takes or gives back
+  int free;     // free pages before the call
+  int by_rows;  // the requests' own threads have written every slot (extend)
+  int pad;
 };
 
 __device__ __forceinline__ int clamp_count(int n, int P) { return min(max(n, 0), P); }
 
 __device__ __forceinline__ int clip_int(long long x) {
   return x > 0x7fffffffll ? 0x7fffffff : static_cast<int>(x);
+}
+
+// Blocks until the launch before this one has ended and its writes are seen
+// (programmatic dependent launch).
+__device__ __forceinline__ void wait_for_prior_launch() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Inclusive sum over the block of one value per thread; *total is the block's.
@@ -52,18 +70,15 @@ __device__ __forceinline__ long long block_sum(long long x, long long* sums, lon
   __syncthreads();  // `sums` of the previous call is read
   if (lane == 31) sums[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    long long s = lane < static_cast<int>(blockDim.x >> 5) ? sums[lane] : 0;
+  long long s = lane < static_cast<int>(blockDim.x >> 5) ? sums[lane] : 0;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, s, d);
-      if (lane >= d) s += y;
-    }
-    sums[lane] = s;
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, s, d);
+    if (lane >= d) s += y;
   }
-  __syncthreads();
-  *total = sums[31];
-  return x + (warp ? sums[warp - 1] : 0);
+  *total = __shfl_sync(0xffffffffu, s, 31);
+  const long long before = __shfl_sync(0xffffffffu, s, max(warp - 1, 0));
+  return x + (warp ? before : 0);
 }
 
 // Last row of rows[0, B) whose member `tok` or `page` is <= x (row 0's is 0).
@@ -77,130 +92,6 @@ __device__ __forceinline__ int find_row(const TableRow* rows, int B, int x) {
   return lo;
 }
 
-// Which requests of an extend call are served and where their tokens and pages
-// start: two running sums over the requests, in order, by one block.
-//   e = sum of new tokens (served or not): the packed position of the tokens
-//   c = sum of new pages of the requests that fit their row and the call
-// A request is served if it needs no page or c <= free.
-__device__ __forceinline__ void extend_rows(const int* new_lens, const int* lens, const int* free_count,
-                                            int* granted, int* lens_out, int* free_out,
-                                            TableHead* head, TableRow* rows, int B, int W, int P,
-                                            int page, int T) {
-  __shared__ long long sums[32];
-  const int free = clamp_count(*free_count, P);
-  const long long cap = static_cast<long long>(W) * page;
-  long long tok0 = 0, page0 = 0;
-  int taken = 0;
-  for (int r0 = 0; r0 < B; r0 += kTableThreads) {
-    const int r = r0 + static_cast<int>(threadIdx.x);
-    const int n = r < B ? max(new_lens[r], 0) : 0;
-    const int len = r < B ? lens[r] : 0;
-    long long all;
-    const long long e = tok0 + block_sum(n, sums, &all);
-    tok0 += all;
-    const bool fits = n > 0 && len >= 0 && static_cast<long long>(len) + n <= cap && e <= T;
-    const int p0 = fits ? (len + page - 1) / page : 0;
-    const int want = fits ? static_cast<int>((static_cast<long long>(len) + n + page - 1) / page) - p0 : 0;
-    const long long c = page0 + block_sum(want, sums, &all);
-    page0 += all;
-    const bool ok = fits && (want == 0 || c <= free);
-    if (ok && want) taken = static_cast<int>(c);
-    if (r < B) {
-      rows[r] = TableRow{clip_int(e - n), clip_int(c - want), len, ok ? n : 0};
-      granted[r] = ok ? n : 0;
-      lens_out[r] = len + (ok ? n : 0);
-    }
-  }
-  // pages taken: c of the last served request that takes any
-  __shared__ int most;
-  if (threadIdx.x == 0) most = 0;
-  __syncthreads();
-  taken = __reduce_max_sync(0xffffffffu, taken);
-  if ((threadIdx.x & 31) == 0) atomicMax(&most, taken);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    *head = TableHead{most, free, {0, 0}};
-    *free_out = free - most;
-  }
-}
-
-// The slots of the call's tokens and the new entries of the block table, by
-// threads `first`, `first + step`, ... of the launch. New entries lie behind
-// the entries that this reads (a request's pages so far), so the order of the
-// threads does not matter. A thread takes kSlotRun tokens in a row: one search.
-constexpr int kSlotRun = 4;
-
-__device__ __forceinline__ void extend_fill(const TableHead* head, const TableRow* rows, int* table,
-                                            long long table_stride, const int* free_pages,
-                                            int* slots, int B, int P, int page, int T,
-                                            long long first, long long step) {
-  const int free = head->free, pages = head->pages;
-  for (long long t0 = first * kSlotRun; t0 < T; t0 += step * kSlotRun) {
-    int r = find_row<&TableRow::tok>(rows, B, static_cast<int>(t0));
-    TableRow row = rows[r];
-#pragma unroll
-    for (int i = 0; i < kSlotRun; ++i) {
-      const int t = static_cast<int>(t0) + i;
-      if (t0 + i >= T) break;
-      while (r + 1 < B && rows[r + 1].tok <= t) row = rows[++r];
-      int slot = -1;
-      if (t - row.tok < row.count) {
-        const int pos = row.len + t - row.tok, j = pos / page;
-        const int fresh = j - (row.len + page - 1) / page;  // >= 0: a page of this call
-        const int id = fresh >= 0 ? free_pages[free - 1 - row.page - fresh] : table[r * table_stride + j];
-        if (static_cast<unsigned>(id) < static_cast<unsigned>(P)) slot = id * page + (pos - j * page);
-      }
-      slots[t] = slot;
-    }
-  }
-  for (long long k = first; k < pages; k += step) {
-    const int r = find_row<&TableRow::page>(rows, B, static_cast<int>(k));
-    const TableRow row = rows[r];
-    const int j = (row.len + page - 1) / page + static_cast<int>(k) - row.page;
-    table[r * table_stride + j] = free_pages[free - 1 - k];
-  }
-}
-
-// Which requests of a release call give pages back and where those start.
-__device__ __forceinline__ void release_rows(const unsigned char* finished, const int* lens,
-                                             const int* free_count, int* lens_out, int* free_out,
-                                             TableHead* head, TableRow* rows, int B, int W, int P,
-                                             int page) {
-  __shared__ long long sums[32];
-  const int free = clamp_count(*free_count, P);
-  long long page0 = 0;
-  for (int r0 = 0; r0 < B; r0 += kTableThreads) {
-    const int r = r0 + static_cast<int>(threadIdx.x);
-    const bool done = r < B && finished[r] != 0;
-    const int len = r < B ? lens[r] : 0;
-    const int n = done ? (min(max(len, 0), W * page) + page - 1) / page : 0;
-    long long all;
-    const long long c = page0 + block_sum(n, sums, &all);
-    page0 += all;
-    if (r < B) {
-      rows[r] = TableRow{0, clip_int(c - n), len, n};
-      lens_out[r] = done ? 0 : len;
-    }
-  }
-  if (threadIdx.x == 0) {
-    // more pages than the stack has room for cannot come from one pool: the
-    // rest are dropped
-    const int back = static_cast<int>(min(page0, static_cast<long long>(P - free)));
-    *head = TableHead{back, free, {0, 0}};
-    *free_out = free + back;
-  }
-}
-
-__device__ __forceinline__ void release_fill(const TableHead* head, const TableRow* rows,
-                                             const int* table, long long table_stride,
-                                             int* free_pages, int B, long long first, long long step) {
-  const int free = head->free, pages = head->pages;
-  for (long long k = first; k < pages; k += step) {
-    const int r = find_row<&TableRow::page>(rows, B, static_cast<int>(k));
-    free_pages[free + k] = table[r * table_stride + (k - rows[r].page)];
-  }
-}
-
 struct ExtendArgs {
   const int *new_lens, *lens, *free_pages, *free_count;
   int *table, *slots, *granted, *lens_out, *free_out;
@@ -210,12 +101,121 @@ struct ExtendArgs {
   int B, W, P, page, T;
 };
 
-__global__ void __launch_bounds__(kTableThreads) extend_kernel(const ExtendArgs a) {
-  extend_rows(a.new_lens, a.lens, a.free_count, a.granted, a.lens_out, a.free_out, a.head, a.rows, a.B,
-              a.W, a.P, a.page, a.T);
+__device__ __forceinline__ int slot_of(int id, int off, const ExtendArgs& a) {
+  return static_cast<unsigned>(id) < static_cast<unsigned>(a.P) ? id * a.page + off : -1;
+}
+
+// Which requests are served and where their tokens and pages start:
+//   e = sum of new tokens (served or not): the packed position of the tokens
+//   c = sum of new pages of the requests that fit their row and the call
+// A request is served if it needs no page or c <= free. A request of few tokens
+// is finished here, with the entry of its last page loaded ahead of the sums.
+// Returns whether a longer one is left to extend_fill.
+__device__ __forceinline__ bool extend_rows(const ExtendArgs& a) {
+  __shared__ long long sums[32];
+  __shared__ int most;
+  if (threadIdx.x == 0) most = 0;
+  const int free = clamp_count(*a.free_count, a.P);
+  const long long cap = static_cast<long long>(a.W) * a.page;
+  long long tok0 = 0, page0 = 0;
+  int taken = 0;
+  bool longer = false;
+  for (int r0 = 0; r0 < a.B; r0 += static_cast<int>(blockDim.x)) {
+    const int r = r0 + static_cast<int>(threadIdx.x);
+    const int n = r < a.B ? max(a.new_lens[r], 0) : 0;
+    const int len = r < a.B ? a.lens[r] : 0;
+    const bool room = n > 0 && len >= 0 && static_cast<long long>(len) + n <= cap;
+    const int p0 = room ? (len + a.page - 1) / a.page : 0;
+    int* row = a.table + static_cast<long long>(r) * a.table_stride;
+    const int last = room && n <= kSlotsByRow && p0 * a.page > len ? row[p0 - 1] : -1;
+    long long all;
+    const long long e = tok0 + block_sum(n, sums, &all);
+    tok0 += all;
+    const bool fits = room && e <= a.T;
+    const int want = fits ? (len + n + a.page - 1) / a.page - p0 : 0;
+    const long long c = page0 + block_sum(want, sums, &all);
+    page0 += all;
+    const bool ok = fits && (want == 0 || c <= free);
+    if (ok && want) taken = static_cast<int>(c);
+    if (r < a.B) {
+      a.rows[r] = TableRow{clip_int(e - n), clip_int(c - want), len, ok ? n : 0};
+      a.granted[r] = ok ? n : 0;
+      a.lens_out[r] = len + (ok ? n : 0);
+    }
+    if (n > kSlotsByRow) {
+      longer = true;
+    } else if (n) {
+      int fresh = -1;
+      if (ok && want) row[p0] = fresh = a.free_pages[free - static_cast<int>(c)];
+#pragma unroll
+      for (int i = 0; i < kSlotsByRow; ++i) {
+        const long long t = e - n + i;
+        if (i >= n || t >= a.T) break;
+        const int pos = len + i, in_new = pos - p0 * a.page;
+        a.slots[t] = !ok ? -1 : in_new >= 0 ? slot_of(fresh, in_new, a) : slot_of(last, in_new + a.page, a);
+      }
+    }
+  }
+  // pages taken: c of the last served request that takes any
+  taken = __reduce_max_sync(0xffffffffu, taken);
+  if ((threadIdx.x & 31) == 0) atomicMax(&most, taken);
+  longer = __syncthreads_or(longer);
+  // no token behind the last; extend_fill writes these too
+  if (!longer)
+    for (long long t = tok0 + threadIdx.x; t < a.T; t += blockDim.x) a.slots[t] = -1;
+  if (threadIdx.x == 0) {
+    *a.head = TableHead{most, free, longer ? 0 : 1, 0};
+    *a.free_out = free - most;
+  }
+  return longer;
+}
+
+// The slots of the call's tokens and the new entries of the block table, by
+// threads `first`, `first + step`, ... of the launch. New entries lie behind
+// the entries that this reads (a request's pages so far), so the order of the
+// threads does not matter. A thread takes kSlotRun tokens in a row: one search.
+constexpr int kSlotRun = 8;
+
+__device__ __forceinline__ void extend_fill(const ExtendArgs& a, long long first, long long step) {
+  const int free = a.head->free, pages = a.head->pages;
+  for (long long t0 = first * kSlotRun; t0 < a.T; t0 += step * kSlotRun) {
+    int r = find_row<&TableRow::tok>(a.rows, a.B, static_cast<int>(t0));
+    TableRow row = a.rows[r];
+#pragma unroll
+    for (int i = 0; i < kSlotRun; ++i) {
+      if (t0 + i >= a.T) break;
+      const int t = static_cast<int>(t0) + i;
+      while (r + 1 < a.B && a.rows[r + 1].tok <= t) row = a.rows[++r];
+      int slot = -1;
+      if (t - row.tok < row.count) {
+        const int pos = row.len + t - row.tok, j = pos / a.page;
+        const int fresh = j - (row.len + a.page - 1) / a.page;  // >= 0: a page of this call
+        const int id = fresh >= 0 ? a.free_pages[free - 1 - row.page - fresh]
+                                  : a.table[r * a.table_stride + j];
+        slot = slot_of(id, pos - j * a.page, a);
+      }
+      a.slots[t] = slot;
+    }
+  }
+  for (long long k = first; k < pages; k += step) {
+    const int r = find_row<&TableRow::page>(a.rows, a.B, static_cast<int>(k));
+    const TableRow row = a.rows[r];
+    const int j = (row.len + a.page - 1) / a.page + static_cast<int>(k) - row.page;
+    a.table[r * a.table_stride + j] = a.free_pages[free - 1 - k];
+  }
+}
+
+__global__ void __launch_bounds__(kTableThreads) extend_kernel(const ExtendArgs a, int fill) {
+  const bool longer = extend_rows(a);
+  if (!fill || !longer) return;
   __syncthreads();
-  extend_fill(a.head, a.rows, a.table, a.table_stride, a.free_pages, a.slots, a.B, a.P, a.page, a.T,
-              threadIdx.x, blockDim.x);
+  extend_fill(a, threadIdx.x, blockDim.x);
+}
+
+__global__ void __launch_bounds__(256) extend_fill_kernel(const ExtendArgs a) {
+  wait_for_prior_launch();
+  if (a.head->by_rows) return;
+  extend_fill(a, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
 }
 
 struct ReleaseArgs {
@@ -228,11 +228,64 @@ struct ReleaseArgs {
   int B, W, P, page;
 };
 
-__global__ void __launch_bounds__(kTableThreads) release_kernel(const ReleaseArgs a) {
-  release_rows(a.finished, a.lens, a.free_count, a.lens_out, a.free_out, a.head, a.rows, a.B, a.W, a.P,
-               a.page);
+// Which requests give pages back and where those start.
+__device__ __forceinline__ void release_rows(const ReleaseArgs& a) {
+  __shared__ long long sums[32];
+  const int free = clamp_count(*a.free_count, a.P);
+  long long page0 = 0;
+  for (int r0 = 0; r0 < a.B; r0 += static_cast<int>(blockDim.x)) {
+    const int r = r0 + static_cast<int>(threadIdx.x);
+    const bool done = r < a.B && a.finished[r] != 0;
+    const int len = r < a.B ? a.lens[r] : 0;
+    const int n = done ? (min(max(len, 0), a.W * a.page) + a.page - 1) / a.page : 0;
+    long long all;
+    const long long c = page0 + block_sum(n, sums, &all);
+    page0 += all;
+    if (r < a.B) {
+      a.rows[r] = TableRow{0, clip_int(c - n), len, n};
+      a.lens_out[r] = done ? 0 : len;
+    }
+  }
+  if (threadIdx.x == 0) {
+    // more pages than the stack has room for cannot come from one pool: the
+    // rest are dropped
+    const int back = static_cast<int>(min(page0, static_cast<long long>(a.P - free)));
+    *a.head = TableHead{back, free, 0, 0};
+    *a.free_out = free + back;
+  }
+}
+
+// The pages onto the stack: warp `first`, `first + step`, ... of the launch each
+// copy up to kReleaseRun entries of a row.
+constexpr int kReleaseRun = 256;
+
+__device__ __forceinline__ void release_fill(const ReleaseArgs& a, long long first, long long step) {
+  const int free = a.head->free, pages = a.head->pages, lane = threadIdx.x & 31;
+  const int runs = (a.W + kReleaseRun - 1) / kReleaseRun;
+  const long long all = static_cast<long long>(a.B) * runs;
+  for (long long i = first; i < all; i += step) {
+    const int r = static_cast<int>(i / runs), j0 = static_cast<int>(i % runs) * kReleaseRun;
+    const TableRow row = a.rows[r];
+    // a clipped first page is behind the stack's end
+    const long long end = min(min(static_cast<long long>(row.count), static_cast<long long>(j0) + kReleaseRun),
+                              static_cast<long long>(pages) - row.page);
+    const int* from = a.table + r * a.table_stride;
+    int* to = a.free_pages + free + row.page;
+#pragma unroll 8
+    for (long long j = j0 + lane; j < end; j += 32) to[j] = from[j];
+  }
+}
+
+__global__ void __launch_bounds__(kTableThreads) release_kernel(const ReleaseArgs a, int fill) {
+  release_rows(a);
+  if (!fill) return;
   __syncthreads();
-  release_fill(a.head, a.rows, a.table, a.table_stride, a.free_pages, a.B, threadIdx.x, blockDim.x);
+  release_fill(a, threadIdx.x >> 5, blockDim.x >> 5);
+}
+
+__global__ void __launch_bounds__(256) release_fill_kernel(const ReleaseArgs a) {
+  wait_for_prior_launch();
+  release_fill(a, blockIdx.x * 8ll + (threadIdx.x >> 5), gridDim.x * 8ll);
 }
 
 // ---------------------------------------------------------------------------
@@ -735,6 +788,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, 
   __shared__ float2 s_ml[kPagedMaxBlocks];
   __shared__ float4 s_o[128];
   __shared__ float s_red[4];
+  wait_for_prior_launch();
   const int4 unit = a.split[blockIdx.x];
   if (unit.x < 0) return;
   const int group = a.Hq / a.Hkv, rt = unit.y % a.row_tiles, head0 = unit.y / a.row_tiles * group;

@@ -237,6 +237,17 @@ int launch_after(void (*kernel)(Params...), const char* name, dim3 grid, int thr
   return launch_status(name);
 }
 
+template <int D>
+int append_launch(const AppendArgs& a, long long rows, int sms, void* stream) {
+  auto s = static_cast<cudaStream_t>(stream);
+  const long long per = 256 / (D / 8);   // rows of a block, one a thread
+  if (rows < 16 * per * sms)
+    append_kernel<D, 1><<<static_cast<unsigned>((rows + per - 1) / per), 256, 0, s>>>(a);
+  else
+    append_kernel<D, 4><<<static_cast<unsigned>((rows + 4 * per - 1) / (4 * per)), 256, 0, s>>>(a);
+  return launch_status("append_kernel");
+}
+
 // Threads of a one-block launch with `work` independent items.
 int table_threads(long long work) {
   return static_cast<int>(std::min<long long>(kTableThreads, std::max<long long>(128, (work + 31) / 32 * 32)));
@@ -260,8 +271,8 @@ int paged_attn_launch(PagedAttnArgs& a, int sms, cudaStream_t stream) {
   const int blocks = static_cast<int>(std::min<double>(std::min(2 * sms, kPagedMaxBlocks), most));
   paged_attn_kernel<D, BF, MT><<<blocks, 128, C::SMEM, stream>>>(a);
   if (int st = launch_status("paged_attn_kernel")) return st;
-  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel", dim3(blocks, std::min(group, 8)),
-                      128, stream, a, 16 * MT);
+  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel", dim3(blocks), kJoinThreads,
+                      stream, a, 16 * MT);
 }
 
 template <int D, bool BF>
@@ -931,7 +942,7 @@ int fa_b200_paged_extend(const int* new_lens, const int* lens, int* block_table,
                           lens_out, free_count_out, table_stride, head,
                           reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size, T};
   auto s = static_cast<cudaStream_t>(stream);
-  const bool wide = T > fab::kTableWide;
+  const bool wide = T > fab::kExtendWide;
   fab::extend_kernel<<<1, fab::table_threads(std::max(B, T / fab::kSlotRun)), 0, s>>>(a, !wide);
   if (int st = fab::launch_status("extend_kernel")) return st;
   if (!wide) return FA_B200_OK;
@@ -963,7 +974,7 @@ int fa_b200_paged_release(const unsigned char* finished, const int* lens, const 
                            reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size};
   auto s = static_cast<cudaStream_t>(stream);
   const long long runs = static_cast<long long>(B) * ((W + fab::kReleaseRun - 1) / fab::kReleaseRun);
-  const bool wide = std::min<long long>(P, static_cast<long long>(B) * W) > fab::kTableWide;
+  const bool wide = std::min<long long>(P, static_cast<long long>(B) * W) > fab::kReleaseWide;
   fab::release_kernel<<<1, fab::table_threads(std::max<long long>(B, wide ? 0 : 32 * runs)), 0, s>>>(a, !wide);
   if (int st = fab::launch_status("release_kernel")) return st;
   if (!wide) return FA_B200_OK;
@@ -991,18 +1002,14 @@ int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b2
       !fab::aligned16(v_cache) || !fab::strides_ok(a.sk, 2) || !fab::strides_ok(a.sv, 2) ||
       !fab::strides_ok(a.skc, 2) || !fab::strides_ok(a.svc, 2))
     return FA_B200_ERR_ALIGNMENT;
-  const long long blocks = (static_cast<long long>(T) * Hkv * (D / 8) + 255) / 256;
-  if (blocks > 0x7fffffffll) return FA_B200_ERR_TOO_LARGE;
+  const long long rows = static_cast<long long>(T) * Hkv;
+  if (rows > (0x7fffffffll << 4)) return FA_B200_ERR_TOO_LARGE;
   if (T == 0) return FA_B200_OK;
-  int dev = 0;
+  int dev = 0, sms = 0;
   int* err = nullptr;
-  if (int st = fab::device_setup(&dev, &err)) return st;
-  auto s = static_cast<cudaStream_t>(stream);
-  if (D == 64)
-    fab::append_kernel<64><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-  else
-    fab::append_kernel<128><<<static_cast<unsigned>(blocks), 256, 0, s>>>(a);
-  return fab::launch_status("append_kernel");
+  if (int st = fab::device_setup(&dev, &err, &sms)) return st;
+  return D == 64 ? fab::append_launch<64>(a, rows, sms, stream)
+                 : fab::append_launch<128>(a, rows, sms, stream);
 }
 
 size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size) {

@@ -23,11 +23,10 @@ namespace fab {
 // writes that need only their results. The sums are latency: a load, two scans,
 // a store. The writes go by the same block where the host knows that they are
 // few, else by a second launch that fills the GPU and whose start overlaps the
-// first (kTableWide).
+// first (kExtendWide, kReleaseWide).
 constexpr int kTableThreads = 1024;
-// Slots (extend) or table entries (release) above which the second launch pays:
-// one block writes about 2 a nanosecond, a launch more costs about 1.5 us.
-constexpr int kTableWide = 8192;
+// Slots (extend) and table entries (release) above which the second launch pays.
+constexpr int kExtendWide = 8192, kReleaseWide = 65536;
 // Up to this many tokens a request's own thread writes them (a decoding step);
 // a page holds 16 or more, so they take at most one new page.
 constexpr int kSlotsByRow = 4;
@@ -81,13 +80,13 @@ __device__ __forceinline__ long long block_sum(long long x, long long* sums, lon
   return x + (warp ? before : 0);
 }
 
-// Last row of rows[0, B) whose member `tok` or `page` is <= x (row 0's is 0).
-template <int TableRow::*M>
-__device__ __forceinline__ int find_row(const TableRow* rows, int B, int x) {
-  int lo = 0, hi = B;  // rows[lo] <= x, rows[hi] > x
+// Last row r of [0, B) with start(r) <= x; start does not fall, start(0) is 0.
+template <typename Start>
+__device__ __forceinline__ int last_at_most(const Start& start, int B, int x) {
+  int lo = 0, hi = B;  // start(lo) <= x < start(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (rows[mid].*M <= x) lo = mid; else hi = mid;
+    if (start(mid) <= x) lo = mid; else hi = mid;
   }
   return lo;
 }
@@ -173,35 +172,80 @@ __device__ __forceinline__ bool extend_rows(const ExtendArgs& a) {
 // The slots of the call's tokens and the new entries of the block table, by
 // threads `first`, `first + step`, ... of the launch. New entries lie behind
 // the entries that this reads (a request's pages so far), so the order of the
-// threads does not matter. A thread takes kSlotRun tokens in a row: one search.
+// threads does not matter. A thread takes kSlotRun tokens in a row: one search
+// and, inside a request, at most two pages (a page holds 16 or more).
 constexpr int kSlotRun = 8;
+constexpr int kRowsShared = 2048;  // rows whose first tokens and pages are searched in shared memory
 
-__device__ __forceinline__ void extend_fill(const ExtendArgs& a, long long first, long long step) {
+// Page of position j * page ... of a row, given its TableRow.
+__device__ __forceinline__ int page_id(const ExtendArgs& a, const TableRow& row, int r, int j, int free) {
+  const int fresh = j - (row.len + a.page - 1) / a.page;  // >= 0: a page of this call
+  return fresh >= 0 ? a.free_pages[free - 1 - row.page - fresh] : a.table[r * a.table_stride + j];
+}
+
+template <typename Tok, typename Page>
+__device__ __forceinline__ void extend_fill(const ExtendArgs& a, const Tok& tok, const Page& page_of,
+                                            long long first, long long step) {
   const int free = a.head->free, pages = a.head->pages;
+  const bool vec = (reinterpret_cast<uintptr_t>(a.slots) & 15) == 0;
   for (long long t0 = first * kSlotRun; t0 < a.T; t0 += step * kSlotRun) {
-    int r = find_row<&TableRow::tok>(a.rows, a.B, static_cast<int>(t0));
+    const int t = static_cast<int>(t0);
+    int r = last_at_most(tok, a.B, t);
     TableRow row = a.rows[r];
+    int slot[kSlotRun];
+    const int in = t - row.tok;
+    if (in + kSlotRun <= row.count) {   // one request
+      const int pos = row.len + in, j = pos / a.page, off = pos - j * a.page;
+      const int id0 = page_id(a, row, r, j, free);
+      const int id1 = off + kSlotRun > a.page ? page_id(a, row, r, j + 1, free) : -1;
 #pragma unroll
-    for (int i = 0; i < kSlotRun; ++i) {
-      if (t0 + i >= a.T) break;
-      const int t = static_cast<int>(t0) + i;
-      while (r + 1 < a.B && a.rows[r + 1].tok <= t) row = a.rows[++r];
-      int slot = -1;
-      if (t - row.tok < row.count) {
-        const int pos = row.len + t - row.tok, j = pos / a.page;
-        const int fresh = j - (row.len + a.page - 1) / a.page;  // >= 0: a page of this call
-        const int id = fresh >= 0 ? a.free_pages[free - 1 - row.page - fresh]
-                                  : a.table[r * a.table_stride + j];
-        slot = slot_of(id, pos - j * a.page, a);
+      for (int i = 0; i < kSlotRun; ++i)
+        slot[i] = off + i < a.page ? slot_of(id0, off + i, a) : slot_of(id1, off + i - a.page, a);
+    } else {
+      for (int i = 0; i < kSlotRun; ++i) {
+        const long long ti = t0 + i;
+        while (r + 1 < a.B && tok(r + 1) <= ti) row = a.rows[++r];
+        const long long at = ti - row.tok;
+        int x = -1;
+        if (at < row.count) {
+          const int pos = row.len + static_cast<int>(at), j = pos / a.page;
+          x = slot_of(page_id(a, row, r, j, free), pos - j * a.page, a);
+        }
+        if (ti < a.T) a.slots[ti] = x;
       }
-      a.slots[t] = slot;
+      continue;
+    }
+    if (vec) {
+      int4* out = reinterpret_cast<int4*>(a.slots + t0);
+      out[0] = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      out[1] = make_int4(slot[4], slot[5], slot[6], slot[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kSlotRun; ++i) a.slots[t0 + i] = slot[i];
     }
   }
   for (long long k = first; k < pages; k += step) {
-    const int r = find_row<&TableRow::page>(a.rows, a.B, static_cast<int>(k));
+    const int r = last_at_most(page_of, a.B, static_cast<int>(k));
     const TableRow row = a.rows[r];
     const int j = (row.len + a.page - 1) / a.page + static_cast<int>(k) - row.page;
     a.table[r * a.table_stride + j] = a.free_pages[free - 1 - k];
+  }
+}
+
+// The block's searches: in shared memory where the rows fit, so that a search
+// costs one round trip to L2 and not one per step.
+__device__ __forceinline__ void extend_fill_block(const ExtendArgs& a, long long first, long long step) {
+  __shared__ int s_tok[kRowsShared], s_page[kRowsShared];
+  if (a.B <= kRowsShared) {
+    for (int r = threadIdx.x; r < a.B; r += blockDim.x) {
+      const int2 x = *reinterpret_cast<const int2*>(a.rows + r);
+      s_tok[r] = x.x;
+      s_page[r] = x.y;
+    }
+    __syncthreads();
+    extend_fill(a, [&](int r) { return s_tok[r]; }, [&](int r) { return s_page[r]; }, first, step);
+  } else {
+    extend_fill(a, [&](int r) { return a.rows[r].tok; }, [&](int r) { return a.rows[r].page; }, first, step);
   }
 }
 
@@ -209,13 +253,13 @@ __global__ void __launch_bounds__(kTableThreads) extend_kernel(const ExtendArgs 
   const bool longer = extend_rows(a);
   if (!fill || !longer) return;
   __syncthreads();
-  extend_fill(a, threadIdx.x, blockDim.x);
+  extend_fill_block(a, threadIdx.x, blockDim.x);
 }
 
 __global__ void __launch_bounds__(256) extend_fill_kernel(const ExtendArgs a) {
   wait_for_prior_launch();
   if (a.head->by_rows) return;
-  extend_fill(a, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
+  extend_fill_block(a, blockIdx.x * 256ll + threadIdx.x, gridDim.x * 256ll);
 }
 
 struct ReleaseArgs {
@@ -264,8 +308,9 @@ __device__ __forceinline__ void release_fill(const ReleaseArgs& a, long long fir
   const int runs = (a.W + kReleaseRun - 1) / kReleaseRun;
   const long long all = static_cast<long long>(a.B) * runs;
   for (long long i = first; i < all; i += step) {
-    const int r = static_cast<int>(i / runs), j0 = static_cast<int>(i % runs) * kReleaseRun;
+    const int r = static_cast<int>(i / runs), j0 = static_cast<int>(i - static_cast<long long>(r) * runs) * kReleaseRun;
     const TableRow row = a.rows[r];
+    if (j0 >= row.count) continue;
     // a clipped first page is behind the stack's end
     const long long end = min(min(static_cast<long long>(row.count), static_cast<long long>(j0) + kReleaseRun),
                               static_cast<long long>(pages) - row.page);
@@ -299,21 +344,34 @@ struct AppendArgs {
   int T, Hkv, P, page;
 };
 
-// One 16-byte piece of k and of v per thread.
-template <int D>
+// A 16-byte piece of k and of v of kAppendRows (token, head) rows per thread, all
+// loads ahead of the stores: 4 rows where that still fills the GPU, else 1. The pieces of a row are neighbouring threads.
+template <int D, int kAppendRows>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
-  const long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  const long long row = i / (D / 8);
-  if (row >= static_cast<long long>(a.T) * a.Hkv) return;
-  const int c = static_cast<int>(i % (D / 8)) * 8;
-  const int t = static_cast<int>(row / a.Hkv), h = static_cast<int>(row % a.Hkv);
-  const int slot = a.slots[t];
-  if (slot < 0 || slot >= a.P * a.page) return;
-  const int id = slot / a.page, off = slot % a.page;
-  *reinterpret_cast<uint4*>(a.k_cache + a.skc.at(id, h, off) + c) =
-      *reinterpret_cast<const uint4*>(a.k + a.sk.at(0, h, t) + c);
-  *reinterpret_cast<uint4*>(a.v_cache + a.svc.at(id, h, off) + c) =
-      *reinterpret_cast<const uint4*>(a.v + a.sv.at(0, h, t) + c);
+  constexpr int CH = D / 8, RPB = 256 / CH;   // pieces of a row, rows a block covers at once
+  const long long rows = static_cast<long long>(a.T) * a.Hkv;
+  const int c = static_cast<int>(threadIdx.x) % CH * 8;
+  const long long row0 = static_cast<long long>(blockIdx.x) * (RPB * kAppendRows) + threadIdx.x / CH;
+  uint4 k[kAppendRows], v[kAppendRows];
+  int slot[kAppendRows], head[kAppendRows];
+#pragma unroll
+  for (int i = 0; i < kAppendRows; ++i) {
+    const long long row = row0 + i * RPB;
+    slot[i] = -1;
+    if (row >= rows) continue;
+    const int t = static_cast<int>(row / a.Hkv);
+    head[i] = static_cast<int>(row - static_cast<long long>(t) * a.Hkv);
+    slot[i] = a.slots[t];
+    k[i] = *reinterpret_cast<const uint4*>(a.k + a.sk.at(0, head[i], t) + c);
+    v[i] = *reinterpret_cast<const uint4*>(a.v + a.sv.at(0, head[i], t) + c);
+  }
+#pragma unroll
+  for (int i = 0; i < kAppendRows; ++i) {
+    if (slot[i] < 0 || slot[i] >= a.P * a.page) continue;
+    const int id = slot[i] / a.page, off = slot[i] - id * a.page;
+    *reinterpret_cast<uint4*>(a.k_cache + a.skc.at(id, head[i], off) + c) = k[i];
+    *reinterpret_cast<uint4*>(a.v_cache + a.svc.at(id, head[i], off) + c) = v[i];
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -503,24 +561,27 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   const uint32_t ring = smem_u32(smem) + warp * C::STAGES * 2 * C::TILE;
   constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows a warp covers at once
   const int lc = lane % CH, lr = lane / CH;
-  int ids[C::GROUPS];
-  PagedAt ld = at;
-  const auto fetch_ids = [&]() {
+  // The next step to load and the one behind it, their pages already looked up.
+  struct Next {
+    PagedAt at;
+    int ids[C::GROUPS];
+  } ld, ld2;
+  const auto fetch_ids = [&](Next& x) {
 #pragma unroll
     for (int g = 0; g < C::GROUPS; ++g) {
-      const int key = ld.t * C::STEP + warp * C::KEYS + g * 16;
-      ids[g] = key < ld.len ? a.table[ld.b * a.table_stride + key / a.page] : 0;
+      const int key = x.at.t * C::STEP + warp * C::KEYS + g * 16;
+      x.ids[g] = key < x.at.len ? a.table[x.at.b * a.table_stride + key / a.page] : 0;
     }
   };
-  const auto issue = [&](int stage) {
+  const auto issue = [&](int stage, const Next& x) {
     const uint32_t kd = ring + stage * 2 * C::TILE + lr * (D * 2);
-    const int kv_head = ld.unit / a.row_tiles;
+    const int kv_head = x.at.unit / a.row_tiles;
     int valid = 0;
 #pragma unroll
     for (int g = 0; g < C::GROUPS; ++g) {
-      const int key = ld.t * C::STEP + warp * C::KEYS + g * 16;
-      int n = min(max(ld.len - key, 0), 16);
-      int id = ids[g];
+      const int key = x.at.t * C::STEP + warp * C::KEYS + g * 16;
+      int n = min(max(x.at.len - key, 0), 16);
+      int id = x.ids[g];
       if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.P)) {
         if (n && lane == 0) atomicCAS(a.err, 0, static_cast<int>(kErrPage));
         n = id = 0;
@@ -542,13 +603,20 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   };
   const long long n_steps = g1 - g0;
   long long issued = 0;
-  fetch_ids();
+  ld.at = at;
+  fetch_ids(ld);
+  ld2.at = at;
+  if (n_steps > 1) {
+    advance(ld2.at);
+    fetch_ids(ld2);
+  }
   const auto issue_next = [&](int stage) {
     if (issued < n_steps) {
-      issue(stage);
-      if (++issued < n_steps) {
-        advance(ld);
-        fetch_ids();
+      issue(stage, ld);
+      ld = ld2;
+      if (++issued + 1 < n_steps) {
+        advance(ld2.at);
+        fetch_ids(ld2);
       }
     }
     cp_async_commit();
@@ -563,22 +631,26 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   constexpr float kBias = BF ? 0.f : 7.f;
   uint32_t qf[MT][D / 16][4];
   float o[MT][D / 8][4], m[MT][2], l[MT][2];
-  const auto begin_unit = [&]() {
-    const int rt = at.unit % a.row_tiles, head0 = at.unit / a.row_tiles * group;
+  const auto load_q = [&](const PagedAt& x) {
+    const int rt = x.unit % a.row_tiles, head0 = x.unit / a.row_tiles * group;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = (rt * MT + mt) * 16 + e * 8 + lane / 4;
-        const uint16_t* q = a.q + a.sq.at(at.b, head0 + min(r, group - 1), 0) + (lane & 3) * 2;
+        const uint16_t* q = a.q + a.sq.at(x.b, head0 + min(r, group - 1), 0) + (lane & 3) * 2;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           qf[mt][ks][e] = r < group ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
           qf[mt][ks][e + 2] = r < group ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
         }
-        m[mt][e] = -INFINITY;
-        l[mt][e] = 0.f;
       }
+  };
+  const auto clear = [&]() {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      m[mt][0] = m[mt][1] = -INFINITY;
+      l[mt][0] = l[mt][1] = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
 #pragma unroll
@@ -597,7 +669,8 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   };
 
   int first_t = at.t;
-  begin_unit();
+  load_q(at);
+  clear();
   int stage = C::STAGES - 1;
   for (long long it = 0; it < n_steps; ++it) {
     const int free_stage = stage;
@@ -691,6 +764,12 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
       ++at.t;
       continue;
     }
+    // the next unit's queries are on their way meanwhile
+    PagedAt next = at;
+    if (it + 1 < n_steps) {
+      advance(next);
+      load_q(next);
+    }
     const bool whole = first_t == 0 && at.t + 1 == at.nt;
     const int rt = at.unit % a.row_tiles, head0 = at.unit / a.row_tiles * group;
 #pragma unroll
@@ -770,83 +849,80 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
       const long long last = g1 - 1 + (at.nt - 1 - at.t);
       a.split[blockIdx.x] = make_int4(at.b, at.unit, static_cast<int>(((last + 1) * blocks - 1) / total), 0);
     }
-    if (it + 1 < n_steps) {
-      advance(at);
-      first_t = 0;
-      begin_unit();
-    }
+    at = next;
+    first_t = 0;
+    clear();
   }
 }
 
 // Adds the parts of the units that a border of paged_attn_kernel cut: block x
-// takes the unit whose first part block x of that launch holds, blocks y its
-// rows in turn. The parts are those of consecutive blocks, so in key order.
+// takes the unit whose first part block x of that launch holds. The parts are
+// those of consecutive blocks, so in key order. A thread owns four columns of a
+// row and every PARTS-th part, each read in one round trip with a running
+// maximum; the threads of a column meet in shared memory.
+constexpr int kJoinThreads = 256;
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedAttnArgs a, int row_tile) {
-  constexpr int COLS = D / 4, PARTS = 128 / COLS;
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int row_tile) {
   constexpr float kBias = BF ? 0.f : 7.f;
-  __shared__ float2 s_ml[kPagedMaxBlocks];
-  __shared__ float4 s_o[128];
-  __shared__ float s_red[4];
+  __shared__ float4 s_o[kJoinThreads];
+  __shared__ float2 s_ml[kJoinThreads];
   wait_for_prior_launch();
   const int4 unit = a.split[blockIdx.x];
   if (unit.x < 0) return;
   const int group = a.Hq / a.Hkv, rt = unit.y % a.row_tiles, head0 = unit.y / a.row_tiles * group;
   const int rows = min(group, row_tile), n = unit.z - static_cast<int>(blockIdx.x) + 1;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int col = threadIdx.x % COLS, part = threadIdx.x / COLS;
-  // part i is the second partial result of the first block, the first one of the others
-  const auto slot = [&](int i, int r) {
-    return (2ll * (blockIdx.x + i) + (i == 0)) * rows + r;
-  };
-  for (int r = blockIdx.y; r < rows && rt * row_tile + r < group; r += gridDim.y) {
-    __syncthreads();
-    float top = -INFINITY;
-    for (int i = threadIdx.x; i < n; i += 128) {
-      const float2 x = a.part_ml[slot(i, r)];
-      s_ml[i] = x;
-      top = fmaxf(top, x.x);
-    }
+  const int here = min(rows, group - rt * row_tile);
+  const int cols = here * (D / 4);
+  // as many threads a column as give each up to four parts
+  const int width = min(cols, kJoinThreads), parts = min(kJoinThreads / width, (n + 3) / 4);
+  const int part = threadIdx.x / width;
+  for (int c0 = 0; c0 < cols; c0 += width) {
+    const int c = c0 + static_cast<int>(threadIdx.x) % width, r = c / (D / 4), col = c % (D / 4) * 4;
+    const bool mine = part < parts && c < cols;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const auto add = [&](float2 ml, float4 x) {
+      const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+      const float w = exp2f(m - ref), y = exp2f(ml.x - ref);
+      m = mn;
+      l = l * w + ml.y * y;
+      o.x = o.x * w + x.x * y;
+      o.y = o.y * w + x.y * y;
+      o.z = o.z * w + x.z * y;
+      o.w = o.w * w + x.w * y;
+    };
+    if (mine) {
+      // part i is the second partial result of the first block, the first one of the others
+      for (int i0 = part; i0 < n; i0 += 4 * parts) {
+        float2 ml[4];
+        float4 x[4];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    if (lane == 0) s_red[warp] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = part; i < n; i += PARTS) {
-      const float4 x = *reinterpret_cast<const float4*>(a.part_o + slot(i, r) * D + col * 4);
-      const float w = exp2f(s_ml[i].x - ref);
-      sum += s_ml[i].y * w;
-      acc.x += x.x * w;
-      acc.y += x.y * w;
-      acc.z += x.z * w;
-      acc.w += x.w * w;
-    }
-    s_o[threadIdx.x] = acc;
-    __syncthreads();
-    if (col == 0) s_ml[part].y = sum;   // s_ml is read
-    __syncthreads();
-    if (part == 0) {
-      sum = s_ml[0].y;
+        for (int j = 0; j < 4; ++j) {
+          const int i = i0 + j * parts;
+          const long long slot = (2ll * (blockIdx.x + min(i, n - 1)) + (i == 0)) * rows + r;
+          ml[j] = i < n ? a.part_ml[slot] : make_float2(-INFINITY, 0.f);
+          x[j] = i < n ? *reinterpret_cast<const float4*>(a.part_o + slot * D + col)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
 #pragma unroll
-      for (int i = 1; i < PARTS; ++i) {
-        const float4 x = s_o[i * COLS + col];
-        acc.x += x.x;
-        acc.y += x.y;
-        acc.z += x.z;
-        acc.w += x.w;
-        sum += s_ml[i].y;
+        for (int j = 0; j < 4; ++j)
+          if (i0 + j * parts < n) add(ml[j], x[j]);
       }
-      const float inv = 1.f / sum;
-      const int head = head0 + rt * row_tile + r;
-      *reinterpret_cast<uint2*>(a.o + a.so.at(unit.x, head, 0) + col * 4) =
-          make_uint2(pack16<BF>(acc.x * inv, acc.y * inv), pack16<BF>(acc.z * inv, acc.w * inv));
-      if (col == 0)
-        a.lse[static_cast<long long>(unit.x) * a.Hq + head] = 0.6931471805599453f * (top - kBias + log2f(sum));
+      s_o[threadIdx.x] = o;
+      s_ml[threadIdx.x] = make_float2(m, l);
     }
+    __syncthreads();
+    if (mine && part == 0) {
+      for (int p = 1; p < parts; ++p) add(s_ml[p * width + threadIdx.x], s_o[p * width + threadIdx.x]);
+      const float inv = 1.f / l;
+      const int head = head0 + rt * row_tile + r;
+      *reinterpret_cast<uint2*>(a.o + a.so.at(unit.x, head, 0) + col) =
+          make_uint2(pack16<BF>(o.x * inv, o.y * inv), pack16<BF>(o.z * inv, o.w * inv));
+      if (col == 0)
+        a.lse[static_cast<long long>(unit.x) * a.Hq + head] = 0.6931471805599453f * (m - kBias + log2f(l));
+    }
+    __syncthreads();
   }
 }
 

@@ -154,7 +154,7 @@ def _outputs(lens, lens_out, free_count_out, *sizes):
     B = lens.numel()
     sizes = (4 * B + 4, *sizes, *(() if lens_out is not None else (B,)),
              *(() if free_count_out is not None else (1,)))
-    ws, *out = lens.new_empty(sum(sizes)).split(sizes)
+    ws, *out = lens.new_empty(sum(sizes)).unsafe_split_with_sizes(sizes)
     if free_count_out is None:
         free_count_out = out.pop()
     else:

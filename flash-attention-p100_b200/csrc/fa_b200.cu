@@ -80,6 +80,15 @@ void set_smem(K kernel, int bytes) {
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+// The paged attention's two cuts; its clusters may have 16 blocks.
+template <int D, bool BF, int ROWS>
+void set_smem_paged() {
+  set_smem(paged_attn_kernel<D, BF, ROWS, false>, PagedCfg<D>::SMEM);
+  set_smem(paged_attn_kernel<D, BF, ROWS, true>, PagedCfg<D>::SMEM);
+  cudaFuncSetAttribute(paged_attn_kernel<D, BF, ROWS, true>,
+                       cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
+
 // Opt every kernel of one element type (fp16, or bf16 when BF) in to its
 // dynamic shared memory.
 template <bool BF>
@@ -94,10 +103,12 @@ void set_smem_all() {
   set_smem(bwd_dq_kernel<128, BF>, DqCfg<128>::SMEM);
   set_smem(bwd_fused_kernel<64, BF>, FusedCfg<64>::SMEM);
   set_smem(bwd_fused_kernel<128, BF>, FusedCfg<128>::SMEM);
-  set_smem(paged_attn_kernel<64, BF, 1>, PagedCfg<64>::SMEM);
-  set_smem(paged_attn_kernel<64, BF, 2>, PagedCfg<64>::SMEM);
-  set_smem(paged_attn_kernel<128, BF, 1>, PagedCfg<128>::SMEM);
-  set_smem(paged_attn_kernel<128, BF, 2>, PagedCfg<128>::SMEM);
+  set_smem_paged<64, BF, 8>();
+  set_smem_paged<64, BF, 16>();
+  set_smem_paged<64, BF, 32>();
+  set_smem_paged<128, BF, 8>();
+  set_smem_paged<128, BF, 16>();
+  set_smem_paged<128, BF, 32>();
 }
 
 // One-time, per-device set-up with that device current: architecture check,
@@ -260,32 +271,63 @@ size_t paged_workspace(int group, int D) {
   return kPagedMaxBlocks * sizeof(int4) + rows * (sizeof(float2) + D * sizeof(float));
 }
 
-template <int D, bool BF, int MT>
+// Blocks of a cluster for `units` units whose table rows hold up to `most` steps,
+// 0 where the line is used. Clusters of 16, 8 or 4 blocks that together
+// fill the SMs at most once (two blocks each) and take at most kClusterSteps
+// steps of a full row per block.
+constexpr int kClusterSteps = 8;
+int paged_cluster(long long units, long long most, int sms) {
+  for (int c = 16; c >= 4; c /= 2)
+    if (units * c <= 2 * sms) return most <= static_cast<long long>(c) * kClusterSteps ? c : 0;
+  return 0;
+}
+
+template <int D, bool BF, int ROWS>
 int paged_attn_launch(PagedAttnArgs& a, int sms, cudaStream_t stream) {
   using C = PagedCfg<D>;
   const int group = a.Hq / a.Hkv;
-  a.row_tiles = (group + 16 * MT - 1) / (16 * MT);
+  a.row_tiles = (group + ROWS - 1) / ROWS;
+  a.step_pages = C::STEP / a.page;
+  a.step_rest = C::STEP % a.page;
+  const long long units = static_cast<long long>(a.B) * a.Hkv * a.row_tiles;
+  const long long most = (a.W * a.page + C::STEP - 1) / C::STEP;
+  if (const int c = paged_cluster(units, most, sms)) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = c;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(units * c));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    (void)cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, BF, ROWS, true>, a);
+    return launch_status("paged_attn_kernel (clusters)");
+  }
   // two blocks an SM, fewer where the table has no room for so many steps
-  const double most = static_cast<double>(a.B) * a.Hkv * a.row_tiles *
-                      ((a.W * a.page + C::STEP - 1) / C::STEP);
-  const int blocks = static_cast<int>(std::min<double>(std::min(2 * sms, kPagedMaxBlocks), most));
-  paged_attn_kernel<D, BF, MT><<<blocks, 128, C::SMEM, stream>>>(a);
+  const int blocks = static_cast<int>(std::min<double>(std::min(2 * sms, kPagedMaxBlocks),
+                                                       static_cast<double>(units) * most));
+  paged_attn_kernel<D, BF, ROWS, false><<<blocks, 128, C::SMEM, stream>>>(a);
   if (int st = launch_status("paged_attn_kernel")) return st;
   return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel", dim3(blocks), kJoinThreads,
-                      stream, a, 16 * MT);
+                      stream, a, ROWS);
 }
 
 template <int D, bool BF>
 int paged_attn_impl(PagedAttnArgs& a, void* workspace, void* stream) {
   int dev = 0, sms = 0;
   if (int st = device_setup(&dev, &a.err, &sms)) return st;
-  const size_t rows = 2 * static_cast<size_t>(std::min(a.Hq / a.Hkv, 32)) * kPagedMaxBlocks;
+  const int group = a.Hq / a.Hkv;
+  const size_t rows = 2 * static_cast<size_t>(std::min(group, 32)) * kPagedMaxBlocks;
   a.split = static_cast<int4*>(workspace);
   a.part_o = reinterpret_cast<float*>(a.split + kPagedMaxBlocks);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
   auto s = static_cast<cudaStream_t>(stream);
-  return a.Hq / a.Hkv <= 16 ? paged_attn_launch<D, BF, 1>(a, sms, s)
-                            : paged_attn_launch<D, BF, 2>(a, sms, s);
+  if (group <= 8) return paged_attn_launch<D, BF, 8>(a, sms, s);
+  if (group <= 16) return paged_attn_launch<D, BF, 16>(a, sms, s);
+  return paged_attn_launch<D, BF, 32>(a, sms, s);
 }
 
 // An fp32 dQ is produced by the fused kernel: one pass, dQ added into the

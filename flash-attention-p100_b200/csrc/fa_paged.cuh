@@ -384,14 +384,19 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // 16 heads fills one m16 fragment (a tcgen05 tile would be 128 rows), operands
 // come straight out of the loaded tile, and no accumulator leaves registers.
 //
-// Work is cut along the keys, not along requests: all (request, kv head, row
-// tile) units in order, each as steps of STEP keys, form one line of steps that
-// is divided evenly over the blocks of the launch. A block walks its stretch
-// through unit after unit; a unit that lies within one stretch is finished
-// there, one cut by a border is left as partial results (o, max, sum in fp32)
-// that paged_join_kernel adds up in the order of the keys. So one long request
-// and a thousand ragged ones both keep every SM loading, and the result does not
-// depend on timing.
+// A unit is one request's kv head and a tile of up to ROWS of its query heads;
+// its keys are taken in steps of STEP. The steps are cut along the keys in one
+// of two ways:
+//   * the line (CLUSTER false): all units in order form one line of steps that
+//     is divided evenly over the blocks of the launch. A block walks its stretch
+//     through unit after unit; a unit that lies within one stretch is finished
+//     there, one cut by a border is left as partial results (o, max, sum in
+//     fp32) that paged_join_kernel adds up in the order of the keys. So one long
+//     request and a thousand ragged ones both keep every SM loading;
+//   * clusters (CLUSTER true): the blocks of a cluster share one unit and meet in
+//     distributed shared memory. No sums over the requests ahead, no second
+//     launch: for few and short units, where those are most of the time.
+// Either way the result does not depend on timing.
 //
 // Inside a block each warp takes KEYS of a step's keys into a ring of its own
 // (cp.async, 16 bytes a lane), three steps deep, across unit borders too: the
@@ -404,9 +409,10 @@ struct PagedAttnArgs {
   const int *table, *lens;
   long long table_stride;
   int B, Hq, Hkv, P, W, page;
-  int row_tiles;   // row tiles of 16 * MT heads in a group
+  int row_tiles;              // tiles of ROWS heads in a group
+  int step_pages, step_rest;  // STEP = step_pages * page + step_rest
   float scale;     // log2(e) / sqrt(D)
-  int4* split;     // per block: the unit whose first part it holds (b, unit in b, last block), x < 0: none
+  int4* split;     // per block: the unit whose first part it holds (b, kv head, row tile, last block), x < 0: none
   float2* part_ml; // per block two partial results: [2 block + first][row] max and sum
   float* part_o;   // ... and [2 block + first][row][D]
   int* err;
@@ -425,8 +431,12 @@ struct PagedCfg {
   static constexpr int SMEM = RING + 2 * MERGE;
 };
 
-constexpr int kPagedMaxBlocks = 320;  // blocks of a launch at most: sizes the workspace
+constexpr int kPagedMaxBlocks = 320;  // blocks of a line at most: sizes the workspace
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// `bytes` of the 16 are read, the rest is filled with zeros
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -470,33 +480,165 @@ __device__ __forceinline__ uint32_t pack16(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(addr) : "memory");
+  return x;
+}
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+  float2 x;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(addr) : "memory");
+  return x;
+}
+
+// A running softmax of four columns: folds in a part with maximum and sum ml
+// and unnormalised columns x.
+struct PartSum {
+  float m = -INFINITY, l = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void add(float2 ml, float4 x) {
+    const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+    const float w = ex2(m - ref), y = ex2(ml.x - ref);
+    m = mn;
+    l = l * w + ml.y * y;
+    o.x = o.x * w + x.x * y;
+    o.y = o.y * w + x.y * y;
+    o.z = o.z * w + x.z * y;
+    o.w = o.w * w + x.w * y;
+  }
+};
+
+// Weights are 2^(s - m + bias): m is the running maximum when it last grew by
+// more than 2^8 (scaling o and l only then), and in fp16 the bias keeps weights
+// down to 2^-21 of the largest out of the subnormals (they end at 2^15).
+template <bool BF>
+__device__ __forceinline__ constexpr float weight_bias() { return BF ? 0.f : 7.f; }
+
+// Writes columns col .. col + 3 of a head's result.
+template <bool BF>
+__device__ __forceinline__ void store_part_sum(const PagedAttnArgs& a, const PartSum& x, int b, int head, int col) {
+  const float inv = 1.f / x.l;
+  *reinterpret_cast<uint2*>(a.o + a.so.at(b, head, 0) + col) =
+      make_uint2(pack16<BF>(x.o.x * inv, x.o.y * inv), pack16<BF>(x.o.z * inv, x.o.w * inv));
+  if (col == 0)
+    a.lse[static_cast<long long>(b) * a.Hq + head] = 0.6931471805599453f * (x.m - weight_bias<BF>() + log2f(x.l));
+}
+
+// Adds the warps' results of a unit into warp 0's registers, fragment by fragment
+// (warps 2 and 3 hand theirs to 0 and 1, then 1 to 0), and calls done(fragment) in
+// warp 0. `buf` holds two fragments. Ends with other warps ahead of warp 0.
+template <typename C, int E, int MT, int N, typename Done>
+__device__ __forceinline__ void merge_warps(unsigned char* buf, float2 (&s_ml)[C::WARPS][16], float (&o)[MT][N][4],
+                                            float (&m)[MT][E], float (&l)[MT][E], const Done& done) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
+      l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
+    }
+#pragma unroll
+    for (int half = C::WARPS / 2; half >= 1; half >>= 1) {
+      __syncthreads();   // buf and s_ml are free
+      if (warp >= half && warp < 2 * half) {
+        float2* mine = reinterpret_cast<float2*>(buf + (warp - half) * C::MERGE);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            mine[(i * E + e) * 32 + lane] = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if ((lane & 3) == 0) s_ml[warp][lane / 4 + 8 * e] = make_float2(m[mt][e], l[mt][e]);
+      }
+      __syncthreads();
+      if (warp < half) {
+        const float2* other = reinterpret_cast<const float2*>(buf + warp * C::MERGE);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float2 x = s_ml[warp + half][lane / 4 + 8 * e];
+          const float mn = fmaxf(m[mt][e], x.x);
+          const float w = mn == -INFINITY ? 1.f : ex2(m[mt][e] - mn);
+          const float y = mn == -INFINITY ? 1.f : ex2(x.x - mn);
+          m[mt][e] = mn;
+          l[mt][e] = l[mt][e] * w + x.y * y;
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float2 z = other[(i * E + e) * 32 + lane];
+            o[mt][i][2 * e] = o[mt][i][2 * e] * w + z.x * y;
+            o[mt][i][2 * e + 1] = o[mt][i][2 * e + 1] * w + z.y * y;
+          }
+        }
+      }
+    }
+    if (warp == 0) done(mt);
+  }
+}
+
 // A place on the line of steps.
 struct PagedAt {
-  int b, unit;  // request; kv head * row_tiles + row tile
-  int t, nt;    // step of the unit, steps of the unit
+  int b, head, rt;  // request, kv head, row tile
+  int t, nt;        // step of the unit, steps of the unit
   int len;
 };
 
-// MT m16 fragments of heads per block: 1 up to 16 heads a group, 2 above (a
-// group above 32 is cut into row tiles, each of which reads the cache again).
-template <int D, bool BF, int MT>
+// ROWS query heads of a group per unit: 8 (the lower half of an m16 fragment,
+// half the softmax), 16 (one fragment) or 32 (two); a group above 32 is cut into
+// row tiles, each of which reads the cache again.
+template <int D, bool BF, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) {
   using C = PagedCfg<D>;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ long long s_sum[C::WARPS];
+  constexpr int MT = ROWS > 16 ? 2 : 1, E = ROWS == 8 ? 1 : 2;  // fragments, rows a thread holds of each
+  constexpr float kBias = weight_bias<BF>();
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ long long s_sum[C::WARPS], s_at;
   __shared__ int s_b, s_valid[C::WARPS][C::STAGES];
-  __shared__ long long s_at;
   __shared__ float2 s_ml[C::WARPS][16];
+  __shared__ float2 s_unit_ml[ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
   const int cap = a.W * a.page;
   const auto length = [&](int b) { return min(max(a.lens[b], 0), cap); };
   const auto steps = [&](int len) { return (len + C::STEP - 1) / C::STEP; };
+  const auto empty_row = [&](int b, int head0, int heads) {
+    for (int i = threadIdx.x; i < heads * (D / 2); i += 128)
+      *reinterpret_cast<uint32_t*>(a.o + a.so.at(b, head0 + i / (D / 2), 0) + i % (D / 2) * 2) = 0;
+    for (int h = threadIdx.x; h < heads; h += 128)
+      a.lse[static_cast<long long>(b) * a.Hq + head0 + h] = -INFINITY;
+  };
 
-  // ---- this block's stretch [g0, g1) of the line; every block adds up the lengths itself ----
-  long long total, g0, g1;
-  int blocks;
-  {
+  // ---- this block's steps ----
+  PagedAt at;
+  long long n_steps, total = 0, g1 = 0;
+  int blocks = 0, rank = 0, ranks = 1;
+  if constexpr (CLUSTER) {
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
+    const int unit = blockIdx.x / ranks;
+    at.b = unit / units;
+    at.head = (unit - at.b * units) / a.row_tiles;
+    at.rt = unit % a.row_tiles;
+    at.len = length(at.b);
+    if (at.len == 0) {   // the whole cluster
+      const int head0 = at.head * group + at.rt * ROWS;
+      if (rank == 0) empty_row(at.b, head0, min(ROWS, group - at.rt * ROWS));
+      return;
+    }
+    at.nt = steps(at.len);
+    at.t = static_cast<int>(static_cast<long long>(at.nt) * rank / ranks);
+    n_steps = static_cast<int>(static_cast<long long>(at.nt) * (rank + 1) / ranks) - at.t;
+  } else {
+    // every block adds up the lengths itself; [g0, g1) is its stretch of the line
     const int per = (a.B + 127) / 128;
     const int b0 = min(static_cast<int>(threadIdx.x) * per, a.B), b1 = min(b0 + per, a.B);
     long long mine = 0;
@@ -509,7 +651,6 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     }
     if (lane == 31) s_sum[warp] = sum;
     __syncthreads();
-    total = 0;
 #pragma unroll
     for (int w = 0; w < C::WARPS; ++w) {
       if (w < warp) sum += s_sum[w];
@@ -517,97 +658,126 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     }
     blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
     const int c = blockIdx.x;
-    g0 = c < blocks ? c * total / blocks : total;
+    const long long g0 = c < blocks ? c * total / blocks : total;
     g1 = c < blocks ? (c + 1) * total / blocks : total;
-    long long at = sum - mine;
-    if (at <= g0 && g0 < sum) {
+    n_steps = g1 - g0;
+    long long first = sum - mine;
+    if (first <= g0 && g0 < sum) {
       int b = b0;
       for (;; ++b) {
         const long long n = static_cast<long long>(steps(length(b))) * units;
-        if (g0 < at + n) break;
-        at += n;
+        if (g0 < first + n) break;
+        first += n;
       }
       s_b = b;
-      s_at = g0 - at;
+      s_at = g0 - first;
     }
+    if (threadIdx.x == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+      if (length(b) == 0) empty_row(b, 0, a.Hq);
+    __syncthreads();
+    if (n_steps == 0) return;
+    at.b = s_b;
+    at.len = length(at.b);
+    at.nt = steps(at.len);
+    const int unit = static_cast<int>(s_at / at.nt);
+    at.t = static_cast<int>(s_at - static_cast<long long>(unit) * at.nt);
+    at.head = unit / a.row_tiles;
+    at.rt = unit - at.head * a.row_tiles;
   }
-  if (threadIdx.x == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  // rows without a token
-  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (length(b) != 0) continue;
-    for (int i = threadIdx.x; i < a.Hq * (D / 2); i += 128)
-      *reinterpret_cast<uint32_t*>(a.o + a.so.at(b, i / (D / 2), 0) + i % (D / 2) * 2) = 0;
-    for (int h = threadIdx.x; h < a.Hq; h += 128) a.lse[static_cast<long long>(b) * a.Hq + h] = -INFINITY;
-  }
-  __syncthreads();
-  if (g0 == g1) return;
-
-  PagedAt at;
-  at.b = s_b;
-  at.len = length(at.b);
-  at.nt = steps(at.len);
-  at.unit = static_cast<int>(s_at / at.nt);
-  at.t = static_cast<int>(s_at % at.nt);
-  const auto advance = [&](PagedAt& x) {
-    if (++x.t < x.nt) return;
+  const auto next_unit = [&](PagedAt& x) {
     x.t = 0;
-    if (++x.unit < units) return;
-    x.unit = 0;
+    if (++x.rt < a.row_tiles) return;
+    x.rt = 0;
+    if (++x.head < a.Hkv) return;
+    x.head = 0;
     do x.len = length(++x.b); while (x.len == 0);
     x.nt = steps(x.len);
   };
 
   // ---- loads ----
-  const uint32_t ring = smem_u32(smem) + warp * C::STAGES * 2 * C::TILE;
   constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows a warp covers at once
   const int lc = lane % CH, lr = lane / CH;
+  const uint32_t ring = smem_u32(smem) + warp * C::STAGES * 2 * C::TILE;
+  // piece c of row r lies at r * 2 D + ((c ^ (r & 7)) << 4): RPI rows further on the
+  // xor changes by a constant
+  const uint32_t ring_lane = ring + lr * (D * 2) + ((lc ^ lr) << 4);
+  const int key_w = warp * C::KEYS, page_w = key_w / a.page, off_w = key_w - page_w * a.page;
   // The next step to load and the one behind it, their pages already looked up.
   struct Next {
     PagedAt at;
+    int page, off;      // of the warp's first key
     int ids[C::GROUPS];
   } ld, ld2;
   const auto fetch_ids = [&](Next& x) {
+    const int* row = a.table + x.at.b * a.table_stride;
 #pragma unroll
     for (int g = 0; g < C::GROUPS; ++g) {
-      const int key = x.at.t * C::STEP + warp * C::KEYS + g * 16;
-      x.ids[g] = key < x.at.len ? a.table[x.at.b * a.table_stride + key / a.page] : 0;
+      const int past = x.off + g * 16 >= a.page;   // a page holds 16 or more
+      x.ids[g] = x.at.t * C::STEP + key_w + g * 16 < x.at.len ? row[x.page + past] : 0;
+    }
+  };
+  const auto advance = [&](Next& x) {
+    if (++x.at.t < x.at.nt) {
+      x.page += a.step_pages;
+      x.off += a.step_rest;
+      if (x.off >= a.page) {
+        x.off -= a.page;
+        ++x.page;
+      }
+    } else {
+      next_unit(x.at);
+      x.page = page_w;
+      x.off = off_w;
     }
   };
   const auto issue = [&](int stage, const Next& x) {
-    const uint32_t kd = ring + stage * 2 * C::TILE + lr * (D * 2);
-    const int kv_head = x.at.unit / a.row_tiles;
+    const uint32_t dst = ring_lane + stage * 2 * C::TILE;
+    const int left = x.at.len - (x.at.t * C::STEP + key_w);
     int valid = 0;
 #pragma unroll
     for (int g = 0; g < C::GROUPS; ++g) {
-      const int key = x.at.t * C::STEP + warp * C::KEYS + g * 16;
-      int n = min(max(x.at.len - key, 0), 16);
-      int id = x.ids[g];
+      int n = min(max(left - g * 16, 0), 16), id = x.ids[g];
       if (static_cast<unsigned>(id) >= static_cast<unsigned>(a.P)) {
         if (n && lane == 0) atomicCAS(a.err, 0, static_cast<int>(kErrPage));
         n = id = 0;
       }
       valid |= n << (8 * g);
-      const int off = n ? key % a.page : 0;
-      const uint16_t* k = a.k_cache + a.skc.at(id, kv_head, off + lr) + lc * 8;
-      const uint16_t* v = a.v_cache + a.svc.at(id, kv_head, off + lr) + lc * 8;
+      int off = x.off + g * 16;
+      if (off >= a.page) off -= a.page;
+      const uint16_t* k = a.k_cache + a.skc.at(id, x.at.head, off + lr) + lc * 8;
+      const uint16_t* v = a.v_cache + a.svc.at(id, x.at.head, off + lr) + lc * 8;
+      const uint32_t d = dst + g * 16 * (D * 2);
+      if (n == 16) {
 #pragma unroll
-      for (int i = 0; i < 16 / RPI; ++i) {
-        const int row = i * RPI + lr;           // of the 16
-        const int bytes = row < n ? 16 : 0;     // the rest is filled with zeros, not read
-        const uint32_t dst = kd + (g * 16 + i * RPI) * (D * 2) + ((lc ^ (row & 7)) << 4);
-        cp_async16(dst, k + i * RPI * a.skc.n, bytes);
-        cp_async16(dst + C::TILE, v + i * RPI * a.svc.n, bytes);
+        for (int i = 0; i < 16 / RPI; ++i) {
+          const uint32_t to = (d ^ (((i * RPI) & 7) << 4)) + i * RPI * (D * 2);
+          cp_async16(to, k + i * RPI * a.skc.n);
+          cp_async16(to + C::TILE, v + i * RPI * a.svc.n);
+        }
+      } else if (n > 0) {   // rows behind the last token are filled with zeros, not read
+#pragma unroll
+        for (int i = 0; i < 16 / RPI; ++i) {
+          const uint32_t to = (d ^ (((i * RPI) & 7) << 4)) + i * RPI * (D * 2);
+          const int bytes = i * RPI + lr < n ? 16 : 0;
+          cp_async16(to, k + i * RPI * a.skc.n, bytes);
+          cp_async16(to + C::TILE, v + i * RPI * a.svc.n, bytes);
+        }
       }
     }
     if (lane == 0) s_valid[warp][stage] = valid;
   };
-  const long long n_steps = g1 - g0;
   long long issued = 0;
   ld.at = at;
-  fetch_ids(ld);
-  ld2.at = at;
+  {
+    const long long key = static_cast<long long>(at.t) * C::STEP + key_w;
+    ld.page = static_cast<int>(key / a.page);
+    ld.off = static_cast<int>(key - static_cast<long long>(ld.page) * a.page);
+  }
+  if (n_steps > 0) fetch_ids(ld);
+  ld2 = ld;
   if (n_steps > 1) {
-    advance(ld2.at);
+    advance(ld2);
     fetch_ids(ld2);
   }
   const auto issue_next = [&](int stage) {
@@ -615,7 +785,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
       issue(stage, ld);
       ld = ld2;
       if (++issued + 1 < n_steps) {
-        advance(ld2.at);
+        advance(ld2);
         fetch_ids(ld2);
       }
     }
@@ -625,48 +795,40 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   for (int s = 0; s < C::STAGES - 1; ++s) issue_next(s);
 
   // ---- per unit state ----
-  // Weights are 2^(s - m + kBias): m is the running maximum when it last grew by
-  // more than 2^8 (scaling o and l only then), and in fp16 the bias keeps weights
-  // down to 2^-21 of the largest out of the subnormals (at most 2^15).
-  constexpr float kBias = BF ? 0.f : 7.f;
   uint32_t qf[MT][D / 16][4];
-  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  float o[MT][D / 8][4], m[MT][E], l[MT][E];
   const auto load_q = [&](const PagedAt& x) {
-    const int rt = x.unit % a.row_tiles, head0 = x.unit / a.row_tiles * group;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = (rt * MT + mt) * 16 + e * 8 + lane / 4;
-        const uint16_t* q = a.q + a.sq.at(x.b, head0 + min(r, group - 1), 0) + (lane & 3) * 2;
+        const int r = x.rt * ROWS + mt * 16 + e * 8 + lane / 4;
+        const bool real = e < E && r < group;
+        const uint16_t* q = a.q + a.sq.at(x.b, x.head * group + min(r, group - 1), 0) + (lane & 3) * 2;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
-          qf[mt][ks][e] = r < group ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
-          qf[mt][ks][e + 2] = r < group ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
+          qf[mt][ks][e] = real ? *reinterpret_cast<const uint32_t*>(q + ks * 16) : 0u;
+          qf[mt][ks][e + 2] = real ? *reinterpret_cast<const uint32_t*>(q + ks * 16 + 8) : 0u;
         }
       }
   };
   const auto clear = [&]() {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      m[mt][0] = m[mt][1] = -INFINITY;
-      l[mt][0] = l[mt][1] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        m[mt][e] = -INFINITY;
+        l[mt][e] = 0.f;
+      }
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[mt][i][e] = 0.f;
     }
   };
-  // scales this thread's rows of fragment mt by w[0], w[1]
-  const auto scale_o = [&](int mt, float w0, float w1) {
-#pragma unroll
-    for (int i = 0; i < D / 8; ++i) {
-      o[mt][i][0] *= w0;
-      o[mt][i][1] *= w0;
-      o[mt][i][2] *= w1;
-      o[mt][i][3] *= w1;
-    }
-  };
+  // ldmatrix addresses of a lane inside a run of 16 keys, for columns 0 .. 15
+  const uint32_t k_lane = ((lane >> 4) * 8 + (lane & 7)) * (D * 2) + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+  const uint32_t v_lane = (((lane >> 3) & 1) * 8 + (lane & 7)) * (D * 2) + (((lane >> 4) ^ (lane & 7)) << 4);
 
   int first_t = at.t;
   load_q(at);
@@ -678,6 +840,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     cp_async_wait<C::STAGES - 2>();
     __syncwarp();   // the step's rows are in, and every lane has left the stage before it
     issue_next(free_stage);
+    __syncwarp();   // whole warps from here on
     const int valid = s_valid[warp][stage];
     const uint32_t kt = ring + stage * 2 * C::TILE, vt = kt + C::TILE;
 #pragma unroll
@@ -689,209 +852,192 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mt][0][e] = s[mt][1][e] = 0.f;
-      {
-        const int row = g * 16 + (lane >> 4) * 8 + (lane & 7);
-        const uint32_t base = kt + row * (D * 2);
+      const uint32_t kb = kt + g * 16 * (D * 2) + k_lane;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-          uint32_t f[4];
-          ldsm4(f, base + (((ks * 2 + ((lane >> 3) & 1)) ^ (row & 7)) << 4));
+      for (int ks = 0; ks < D / 16; ++ks) {
+        uint32_t f[4];
+        ldsm4(f, kb ^ (ks << 5));
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16<BF>(s[mt][0], qf[mt][ks], f[0], f[1]);
-            mma16<BF>(s[mt][1], qf[mt][ks], f[2], f[3]);
-          }
+        for (int mt = 0; mt < MT; ++mt) {
+          mma16<BF>(s[mt][0], qf[mt][ks], f[0], f[1]);
+          mma16<BF>(s[mt][1], qf[mt][ks], f[2], f[3]);
         }
+      }
+      if (n < 16) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2 * E; ++e)
+              if (h * 8 + (lane & 3) * 2 + (e & 1) >= n) s[mt][h][e] = -INFINITY;
       }
       uint32_t p[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        float top[2] = {-INFINITY, -INFINITY};
+        float top[E];
+        bool grown = false;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float& x = s[mt][h][e];
-            x = h * 8 + (lane & 3) * 2 + (e & 1) < n ? x * a.scale : -INFINITY;
-            top[e >> 1] = fmaxf(top[e >> 1], x);
-          }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < E; ++e) {
+          top[e] = fmaxf(fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]), fmaxf(s[mt][1][2 * e], s[mt][1][2 * e + 1]));
           top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
+          top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2)) * a.scale;
+          grown |= top[e] > m[mt][e] + 8.f;
         }
-        if (__any_sync(0xffffffffu, top[0] > m[mt][0] + 8.f || top[1] > m[mt][1] + 8.f)) {
-          float w[2];
+        if (__any_sync(0xffffffffu, grown)) {
+          float w[2] = {1.f, 1.f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
+          for (int e = 0; e < E; ++e) {
             const float mn = fmaxf(m[mt][e], top[e]);
-            w[e] = mn == -INFINITY ? 1.f : exp2f(m[mt][e] - mn);
+            w[e] = mn == -INFINITY ? 1.f : ex2(m[mt][e] - mn);
             m[mt][e] = mn;
             l[mt][e] *= w[e];
           }
-          scale_o(mt, w[0], w[1]);
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 2 * E; ++e) o[mt][i][e] *= w[e >> 1];
         }
+        p[mt][1] = p[mt][3] = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+        for (int e = 0; e < E; ++e) {
+          const float ref = m[mt][e] == -INFINITY ? 0.f : kBias - m[mt][e];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float ref = m[mt][e] == -INFINITY ? 0.f : m[mt][e] - kBias;
+          for (int h = 0; h < 2; ++h) {
             // the sum takes the weights as the product with v takes them: rounded
-            const uint32_t w = pack16<BF>(exp2f(s[mt][h][2 * e] - ref), exp2f(s[mt][h][2 * e + 1] - ref));
+            const uint32_t w = pack16<BF>(ex2(fmaf(s[mt][h][2 * e], a.scale, ref)),
+                                          ex2(fmaf(s[mt][h][2 * e + 1], a.scale, ref)));
             const float2 r = unpack16<BF>(w);
             l[mt][e] += r.x + r.y;
             p[mt][2 * h + e] = w;
           }
+        }
       }
-      {
-        const int row = g * 16 + ((lane >> 3) & 1) * 8 + (lane & 7);
-        const uint32_t base = vt + row * (D * 2);
+      const uint32_t vb = vt + g * 16 * (D * 2) + v_lane;
 #pragma unroll
-        for (int dt = 0; dt < D / 16; ++dt) {
-          uint32_t f[4];
-          ldsm4_t(f, base + (((dt * 2 + (lane >> 4)) ^ (row & 7)) << 4));
+      for (int dt = 0; dt < D / 16; ++dt) {
+        uint32_t f[4];
+        ldsm4_t(f, vb ^ (dt << 5));
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma16<BF>(o[mt][2 * dt], p[mt], f[0], f[1]);
-            mma16<BF>(o[mt][2 * dt + 1], p[mt], f[2], f[3]);
-          }
+        for (int mt = 0; mt < MT; ++mt) {
+          mma16<BF>(o[mt][2 * dt], p[mt], f[0], f[1]);
+          mma16<BF>(o[mt][2 * dt + 1], p[mt], f[2], f[3]);
         }
       }
     }
-
-    // ---- end of the unit, or of the stretch: add up the warps ----
-    if (at.t + 1 < at.nt && it + 1 < n_steps) {
+    if (it + 1 < n_steps && (CLUSTER || at.t + 1 < at.nt)) {
       ++at.t;
       continue;
     }
-    // the next unit's queries are on their way meanwhile
-    PagedAt next = at;
-    if (it + 1 < n_steps) {
-      advance(next);
-      load_q(next);
+    if constexpr (CLUSTER) break;
+
+    // ---- the unit's end, or the stretch's ----
+    const PagedAt done = at;
+    if (it + 1 < n_steps) {   // the next unit's queries are on their way meanwhile
+      next_unit(at);
+      load_q(at);
     }
-    const bool whole = first_t == 0 && at.t + 1 == at.nt;
-    const int rt = at.unit % a.row_tiles, head0 = at.unit / a.row_tiles * group;
+    const bool whole = first_t == 0 && done.t + 1 == done.nt;
+    merge_warps<C, E, MT>(smem + C::RING, s_ml, o, m, l, [&](int mt) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
-        l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
-      }
-      float4* buf = reinterpret_cast<float4*>(smem + C::RING);
-      // warps 2 and 3 hand their rows to 0 and 1, then 1 to 0
-#pragma unroll
-      for (int half = C::WARPS / 2; half >= 1; half >>= 1) {
-        __syncthreads();   // the buffers and s_ml are free
-        if (warp >= half && warp < 2 * half) {
-          float4* mine = buf + (warp - half) * (C::MERGE / 16);
+      for (int e = 0; e < E; ++e) {
+        const int row = mt * 16 + e * 8 + lane / 4, r = done.rt * ROWS + row;
+        if (r >= group) continue;
+        const int head = done.head * group + r;
+        if (whole) {
+          const float inv = 1.f / l[mt][e];
+          uint16_t* out = a.o + a.so.at(done.b, head, 0) + (lane & 3) * 2;
 #pragma unroll
           for (int i = 0; i < D / 8; ++i)
-            mine[i * 32 + lane] = make_float4(o[mt][i][0], o[mt][i][1], o[mt][i][2], o[mt][i][3]);
-          if ((lane & 3) == 0) {
-            s_ml[warp][lane / 4] = make_float2(m[mt][0], l[mt][0]);
-            s_ml[warp][lane / 4 + 8] = make_float2(m[mt][1], l[mt][1]);
-          }
-        }
-        __syncthreads();
-        if (warp < half) {
-          float w[2], wo[2];
+            *reinterpret_cast<uint32_t*>(out + i * 8) =
+                pack16<BF>(o[mt][i][2 * e] * inv, o[mt][i][2 * e + 1] * inv);
+          if ((lane & 3) == 0)
+            a.lse[static_cast<long long>(done.b) * a.Hq + head] =
+                0.6931471805599453f * (m[mt][e] - kBias + log2f(l[mt][e]));
+        } else {
+          const long long slot = (2ll * blockIdx.x + (first_t == 0)) * min(group, ROWS) + row;
+          float* out = a.part_o + slot * D + (lane & 3) * 2;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 x = s_ml[warp + half][lane / 4 + 8 * e];
-            const float mn = fmaxf(m[mt][e], x.x);
-            w[e] = mn == -INFINITY ? 1.f : exp2f(m[mt][e] - mn);
-            wo[e] = mn == -INFINITY ? 1.f : exp2f(x.x - mn);
-            m[mt][e] = mn;
-            l[mt][e] = l[mt][e] * w[e] + x.y * wo[e];
-          }
-          const float4* other = buf + warp * (C::MERGE / 16);
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            const float4 x = other[i * 32 + lane];
-            o[mt][i][0] = o[mt][i][0] * w[0] + x.x * wo[0];
-            o[mt][i][1] = o[mt][i][1] * w[0] + x.y * wo[0];
-            o[mt][i][2] = o[mt][i][2] * w[1] + x.z * wo[1];
-            o[mt][i][3] = o[mt][i][3] * w[1] + x.w * wo[1];
-          }
+          for (int i = 0; i < D / 8; ++i)
+            *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+          if ((lane & 3) == 0) a.part_ml[slot] = make_float2(m[mt][e], l[mt][e]);
         }
       }
-      if (warp == 0) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int lr16 = mt * 16 + e * 8 + lane / 4, r = rt * MT * 16 + lr16;
-          if (r >= group) continue;
-          if (whole) {
-            const float inv = 1.f / l[mt][e];
-            uint16_t* out = a.o + a.so.at(at.b, head0 + r, 0) + (lane & 3) * 2;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-              *reinterpret_cast<uint32_t*>(out + i * 8) =
-                  pack16<BF>(o[mt][i][2 * e] * inv, o[mt][i][2 * e + 1] * inv);
-            if ((lane & 3) == 0)
-              a.lse[static_cast<long long>(at.b) * a.Hq + head0 + r] =
-                  0.6931471805599453f * (m[mt][e] - kBias + log2f(l[mt][e]));
-          } else {
-            const int rows = min(group, MT * 16);
-            const long long slot = (2ll * blockIdx.x + (first_t == 0)) * rows + lr16;
-            float* out = a.part_o + slot * D + (lane & 3) * 2;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-              *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
-            if ((lane & 3) == 0) a.part_ml[slot] = make_float2(m[mt][e], l[mt][e]);
-          }
-        }
-      }
-    }
+    });
     if (!whole && first_t == 0 && threadIdx.x == 0) {
       // the block that holds the unit's last step
-      const long long last = g1 - 1 + (at.nt - 1 - at.t);
-      a.split[blockIdx.x] = make_int4(at.b, at.unit, static_cast<int>(((last + 1) * blocks - 1) / total), 0);
+      const long long last = g1 - 1 + (done.nt - 1 - done.t);
+      a.split[blockIdx.x] = make_int4(done.b, done.head, done.rt,
+                                      static_cast<int>(((last + 1) * blocks - 1) / total));
     }
-    at = next;
     first_t = 0;
     clear();
+  }
+
+  if constexpr (CLUSTER) {
+    // this block's part into its shared memory (the ring: every load has landed
+    // and been read), then every block adds up a share of the columns
+    float* part = reinterpret_cast<float*>(smem);
+    merge_warps<C, E, MT>(smem + C::RING, s_ml, o, m, l, [&](int mt) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int row = mt * 16 + e * 8 + lane / 4;
+        float* out = part + row * D + (lane & 3) * 2;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+        if ((lane & 3) == 0) s_unit_ml[row] = make_float2(m[mt][e], l[mt][e]);
+      }
+    });
+    cluster_sync();
+    const int rows = min(ROWS, group - at.rt * ROWS), head0 = at.head * group + at.rt * ROWS;
+    for (int i = rank * 128 + threadIdx.x; i < rows * (D / 4); i += ranks * 128) {
+      const int row = i / (D / 4), col = i % (D / 4) * 4;
+      const uint32_t po = smem_u32(part + row * D + col), pm = smem_u32(&s_unit_ml[row]);
+      PartSum sum;
+      for (int r0 = 0; r0 < ranks; r0 += 4) {   // ranks is a multiple of 4 or less than 4
+        float4 x[4];
+        float2 ml[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int from = min(r0 + r, ranks - 1);
+          x[r] = cluster_load4(cluster_addr(po, from));
+          ml[r] = cluster_load2(cluster_addr(pm, from));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (r0 + r < ranks) sum.add(ml[r], x[r]);
+      }
+      store_part_sum<BF>(a, sum, at.b, head0 + row, col);
+    }
+    cluster_sync();   // no block leaves while another reads its part
   }
 }
 
 // Adds the parts of the units that a border of paged_attn_kernel cut: block x
 // takes the unit whose first part block x of that launch holds. The parts are
 // those of consecutive blocks, so in key order. A thread owns four columns of a
-// row and every PARTS-th part, each read in one round trip with a running
+// row and up to every fourth part, four of them in flight with a running
 // maximum; the threads of a column meet in shared memory.
 constexpr int kJoinThreads = 256;
 
 template <int D, bool BF>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int row_tile) {
-  constexpr float kBias = BF ? 0.f : 7.f;
   __shared__ float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
   wait_for_prior_launch();
   const int4 unit = a.split[blockIdx.x];
   if (unit.x < 0) return;
-  const int group = a.Hq / a.Hkv, rt = unit.y % a.row_tiles, head0 = unit.y / a.row_tiles * group;
-  const int rows = min(group, row_tile), n = unit.z - static_cast<int>(blockIdx.x) + 1;
-  const int here = min(rows, group - rt * row_tile);
-  const int cols = here * (D / 4);
+  const int group = a.Hq / a.Hkv, rows = min(group, row_tile);
+  const int n = unit.w - static_cast<int>(blockIdx.x) + 1;
+  const int cols = min(rows, group - unit.z * row_tile) * (D / 4);
   // as many threads a column as give each up to four parts
   const int width = min(cols, kJoinThreads), parts = min(kJoinThreads / width, (n + 3) / 4);
-  const int part = threadIdx.x / width;
+  const int part = static_cast<int>(threadIdx.x) / width;
   for (int c0 = 0; c0 < cols; c0 += width) {
     const int c = c0 + static_cast<int>(threadIdx.x) % width, r = c / (D / 4), col = c % (D / 4) * 4;
     const bool mine = part < parts && c < cols;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const auto add = [&](float2 ml, float4 x) {
-      const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-      const float w = exp2f(m - ref), y = exp2f(ml.x - ref);
-      m = mn;
-      l = l * w + ml.y * y;
-      o.x = o.x * w + x.x * y;
-      o.y = o.y * w + x.y * y;
-      o.z = o.z * w + x.z * y;
-      o.w = o.w * w + x.w * y;
-    };
+    PartSum sum;
     if (mine) {
       // part i is the second partial result of the first block, the first one of the others
       for (int i0 = part; i0 < n; i0 += 4 * parts) {
@@ -899,28 +1045,22 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
         float4 x[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int i = i0 + j * parts;
-          const long long slot = (2ll * (blockIdx.x + min(i, n - 1)) + (i == 0)) * rows + r;
-          ml[j] = i < n ? a.part_ml[slot] : make_float2(-INFINITY, 0.f);
-          x[j] = i < n ? *reinterpret_cast<const float4*>(a.part_o + slot * D + col)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
+          const int i = min(i0 + j * parts, n - 1);
+          const long long slot = (2ll * (blockIdx.x + i) + (i == 0)) * rows + r;
+          ml[j] = a.part_ml[slot];
+          x[j] = *reinterpret_cast<const float4*>(a.part_o + slot * D + col);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (i0 + j * parts < n) add(ml[j], x[j]);
+          if (i0 + j * parts < n) sum.add(ml[j], x[j]);
       }
-      s_o[threadIdx.x] = o;
-      s_ml[threadIdx.x] = make_float2(m, l);
+      s_o[threadIdx.x] = sum.o;
+      s_ml[threadIdx.x] = make_float2(sum.m, sum.l);
     }
     __syncthreads();
     if (mine && part == 0) {
-      for (int p = 1; p < parts; ++p) add(s_ml[p * width + threadIdx.x], s_o[p * width + threadIdx.x]);
-      const float inv = 1.f / l;
-      const int head = head0 + rt * row_tile + r;
-      *reinterpret_cast<uint2*>(a.o + a.so.at(unit.x, head, 0) + col) =
-          make_uint2(pack16<BF>(o.x * inv, o.y * inv), pack16<BF>(o.z * inv, o.w * inv));
-      if (col == 0)
-        a.lse[static_cast<long long>(unit.x) * a.Hq + head] = 0.6931471805599453f * (m - kBias + log2f(l));
+      for (int p = 1; p < parts; ++p) sum.add(s_ml[p * width + threadIdx.x], s_o[p * width + threadIdx.x]);
+      store_part_sum<BF>(a, sum, unit.x, unit.y * group + unit.z * row_tile + r, col);
     }
     __syncthreads();
   }

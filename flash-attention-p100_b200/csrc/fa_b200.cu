@@ -271,6 +271,15 @@ size_t paged_workspace(int group, int D) {
   return kPagedMaxBlocks * sizeof(int4) + rows * (sizeof(float2) + D * sizeof(float));
 }
 
+// Strides of a cache (16-bit elements, multiples of 8) in units of 16 bytes;
+// false if one does not fit 32 bits. A single page's or head's is not used.
+bool to_units(const Strides& s, int P, int Hkv, Units* u) {
+  const long long b = P > 1 ? s.b / 8 : 0, h = Hkv > 1 ? s.h / 8 : 0, n = s.n / 8;
+  if (std::max({b, h, n}) > 0xffffffffll) return false;
+  *u = Units{static_cast<uint32_t>(b), static_cast<uint32_t>(h), static_cast<uint32_t>(n)};
+  return true;
+}
+
 // Blocks of a cluster for `units` units whose table rows hold up to `most` steps,
 // 0 where the line is used. Clusters of 16, 8 or 4 blocks that together
 // fill the SMs at most once (two blocks each) and take at most kClusterSteps
@@ -1074,18 +1083,20 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
   if (!workspace || workspace_bytes < fab::paged_workspace(Hq / Hkv, D)) return FA_B200_ERR_WORKSPACE;
   fab::PagedAttnArgs a{};
   a.q = static_cast<const uint16_t*>(q);
-  a.k_cache = static_cast<const uint16_t*>(k_cache);
-  a.v_cache = static_cast<const uint16_t*>(v_cache);
+  a.k_cache = static_cast<const uint4*>(k_cache);
+  a.v_cache = static_cast<const uint4*>(v_cache);
   a.o = static_cast<uint16_t*>(o);
   a.lse = lse;
-  a.sq = from_abi(sq), a.so = from_abi(so), a.skc = from_abi(skc), a.svc = from_abi(svc);
+  const fab::Strides sk = from_abi(skc), sv = from_abi(svc);
+  a.sq = from_abi(sq), a.so = from_abi(so);
   a.table = block_table, a.lens = lens, a.table_stride = table_stride;
   a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.P = P, a.W = W, a.page = page_size;
   a.scale = 1.4426950408889634f / sqrtf(static_cast<float>(D));
   if (!fab::aligned16(q) || !fab::aligned16(k_cache) || !fab::aligned16(v_cache) ||
       !fab::aligned16(o) || !fab::aligned16(workspace) || !fab::strides_ok(a.sq, 2) ||
-      !fab::strides_ok(a.so, 2) || !fab::strides_ok(a.skc, 2) || !fab::strides_ok(a.svc, 2))
+      !fab::strides_ok(a.so, 2) || !fab::strides_ok(sk, 2) || !fab::strides_ok(sv, 2))
     return FA_B200_ERR_ALIGNMENT;
+  if (!fab::to_units(sk, P, Hkv, &a.skc) || !fab::to_units(sv, P, Hkv, &a.svc)) return FA_B200_ERR_TOO_LARGE;
   const bool bf = dtype == FA_B200_DTYPE_BF16;
   if (D == 64)
     return bf ? fab::paged_attn_impl<64, true>(a, workspace, stream)

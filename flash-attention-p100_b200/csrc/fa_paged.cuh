@@ -401,11 +401,18 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // Inside a block each warp takes KEYS of a step's keys into a ring of its own
 // (cp.async, 16 bytes a lane), three steps deep, across unit borders too: the
 // loads never drain, and warps meet only where a unit ends.
+// Strides of a cache in units of 16 bytes (page, head, token): products of 32
+// bits, one instruction each, that still span 64 GB.
+struct Units {
+  uint32_t b, h, n;
+};
 struct PagedAttnArgs {
-  const uint16_t *q, *k_cache, *v_cache;
+  const uint16_t* q;
+  const uint4 *k_cache, *v_cache;
   uint16_t* o;
   float* lse;
-  Strides sq, so, skc, svc;  // q, o: b request, h head; caches: b page, h head, n token
+  Strides sq, so;             // b request, h head
+  Units skc, svc;             // of the caches
   const int *table, *lens;
   long long table_stride;
   int B, Hq, Hkv, P, W, page;
@@ -425,6 +432,7 @@ struct PagedCfg {
   static constexpr int KEYS = 2048 / D;       // of a warp in a step: 4 KB of K, 4 KB of V
   static constexpr int STEP = WARPS * KEYS;
   static constexpr int GROUPS = KEYS / 16;    // runs of 16 keys: each lies in one page
+  static constexpr int ALL = GROUPS == 2 ? 0x1010 : 0x10;  // keys of the runs, 8 bits each, when all are real
   static constexpr int TILE = KEYS * D * 2;   // bytes of a warp's K (or V) of a step
   static constexpr int RING = WARPS * STAGES * 2 * TILE;
   static constexpr int MERGE = 16 * D * 4;    // one warp's fp32 result of 16 rows
@@ -583,6 +591,11 @@ __device__ __forceinline__ void merge_warps(unsigned char* buf, float2 (&s_ml)[C
     }
     if (warp == 0) done(mt);
   }
+}
+
+__device__ __forceinline__ const uint4* unit_at(const uint4* base, const Units& s, uint32_t b, uint32_t h,
+                                                uint32_t n) {
+  return base + (static_cast<uint64_t>(b) * s.b + static_cast<uint64_t>(h) * s.h + static_cast<uint64_t>(n) * s.n);
 }
 
 // A place on the line of steps.
@@ -745,8 +758,8 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
       valid |= n << (8 * g);
       int off = x.off + g * 16;
       if (off >= a.page) off -= a.page;
-      const uint16_t* k = a.k_cache + a.skc.at(id, x.at.head, off + lr) + lc * 8;
-      const uint16_t* v = a.v_cache + a.svc.at(id, x.at.head, off + lr) + lc * 8;
+      const uint4* k = unit_at(a.k_cache + lc, a.skc, id, x.at.head, off + lr);
+      const uint4* v = unit_at(a.v_cache + lc, a.svc, id, x.at.head, off + lr);
       const uint32_t d = dst + g * 16 * (D * 2);
       if (n == 16) {
 #pragma unroll
@@ -755,7 +768,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
           cp_async16(to, k + i * RPI * a.skc.n);
           cp_async16(to + C::TILE, v + i * RPI * a.svc.n);
         }
-      } else if (n > 0) {   // rows behind the last token are filled with zeros, not read
+      } else if (left > 0) {   // rows behind the last token are filled with zeros, not read
 #pragma unroll
         for (int i = 0; i < 16 / RPI; ++i) {
           const uint32_t to = (d ^ (((i * RPI) & 7) << 4)) + i * RPI * (D * 2);
@@ -842,44 +855,49 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     issue_next(free_stage);
     __syncwarp();   // whole warps from here on
     const int valid = s_valid[warp][stage];
-    const uint32_t kt = ring + stage * 2 * C::TILE, vt = kt + C::TILE;
-#pragma unroll
-    for (int g = 0; g < C::GROUPS; ++g) {
-      const int n = (valid >> (8 * g)) & 255;
-      if (n == 0) continue;
-      float s[MT][2][4];
+    if (valid != 0) {
+      const uint32_t kb = ring + stage * 2 * C::TILE + k_lane, vb = ring + stage * 2 * C::TILE + C::TILE + v_lane;
+      float s[MT][2 * C::GROUPS][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][0][e] = s[mt][1][e] = 0.f;
-      const uint32_t kb = kt + g * 16 * (D * 2) + k_lane;
+        for (int i = 0; i < 2 * C::GROUPS; ++i)
 #pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        uint32_t f[4];
-        ldsm4(f, kb ^ (ks << 5));
+          for (int e = 0; e < 4; ++e) s[mt][i][e] = 0.f;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16<BF>(s[mt][0], qf[mt][ks], f[0], f[1]);
-          mma16<BF>(s[mt][1], qf[mt][ks], f[2], f[3]);
+      for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+        for (int g = 0; g < C::GROUPS; ++g) {
+          uint32_t f[4];
+          ldsm4(f, (kb ^ (ks << 5)) + g * 16 * (D * 2));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<BF>(s[mt][2 * g], qf[mt][ks], f[0], f[1]);
+            mma16<BF>(s[mt][2 * g + 1], qf[mt][ks], f[2], f[3]);
+          }
         }
-      }
-      if (n < 16) {
+      if (valid != C::ALL) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int i = 0; i < 2 * C::GROUPS; ++i) {
+          const int n = (valid >> (8 * (i >> 1))) & 255, key = (i & 1) * 8 + (lane & 3) * 2;
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int e = 0; e < 2 * E; ++e)
-              if (h * 8 + (lane & 3) * 2 + (e & 1) >= n) s[mt][h][e] = -INFINITY;
+              if (key + (e & 1) >= n) s[mt][i][e] = -INFINITY;
+        }
       }
-      uint32_t p[MT][4];
+      uint32_t p[MT][C::GROUPS][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float top[E];
         bool grown = false;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          top[e] = fmaxf(fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]), fmaxf(s[mt][1][2 * e], s[mt][1][2 * e + 1]));
+          top[e] = fmaxf(s[mt][0][2 * e], s[mt][0][2 * e + 1]);
+#pragma unroll
+          for (int i = 1; i < 2 * C::GROUPS; ++i)
+            top[e] = fmaxf(top[e], fmaxf(s[mt][i][2 * e], s[mt][i][2 * e + 1]));
           top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
           top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2)) * a.scale;
           grown |= top[e] > m[mt][e] + 8.f;
@@ -898,32 +916,33 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
 #pragma unroll
             for (int e = 0; e < 2 * E; ++e) o[mt][i][e] *= w[e >> 1];
         }
-        p[mt][1] = p[mt][3] = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float ref = m[mt][e] == -INFINITY ? 0.f : kBias - m[mt][e];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int i = 0; i < 2 * C::GROUPS; ++i) {
             // the sum takes the weights as the product with v takes them: rounded
-            const uint32_t w = pack16<BF>(ex2(fmaf(s[mt][h][2 * e], a.scale, ref)),
-                                          ex2(fmaf(s[mt][h][2 * e + 1], a.scale, ref)));
+            const uint32_t w = pack16<BF>(ex2(fmaf(s[mt][i][2 * e], a.scale, ref)),
+                                          ex2(fmaf(s[mt][i][2 * e + 1], a.scale, ref)));
             const float2 r = unpack16<BF>(w);
             l[mt][e] += r.x + r.y;
-            p[mt][2 * h + e] = w;
+            p[mt][i >> 1][2 * (i & 1) + e] = w;
+            if (E == 1) p[mt][i >> 1][2 * (i & 1) + 1] = 0;
           }
         }
       }
-      const uint32_t vb = vt + g * 16 * (D * 2) + v_lane;
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) {
-        uint32_t f[4];
-        ldsm4_t(f, vb ^ (dt << 5));
+      for (int g = 0; g < C::GROUPS; ++g)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          mma16<BF>(o[mt][2 * dt], p[mt], f[0], f[1]);
-          mma16<BF>(o[mt][2 * dt + 1], p[mt], f[2], f[3]);
+        for (int dt = 0; dt < D / 16; ++dt) {
+          uint32_t f[4];
+          ldsm4_t(f, (vb ^ (dt << 5)) + g * 16 * (D * 2));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<BF>(o[mt][2 * dt], p[mt][g], f[0], f[1]);
+            mma16<BF>(o[mt][2 * dt + 1], p[mt][g], f[2], f[3]);
+          }
         }
-      }
     }
     if (it + 1 < n_steps && (CLUSTER || at.t + 1 < at.nt)) {
       ++at.t;

@@ -230,33 +230,37 @@ int launch_status(const char* kernel) {
   return FA_B200_ERR_LAUNCH;
 }
 
-// Launches a kernel that waits (griddepcontrol.wait) for the launch before it on
-// `stream`: its blocks are scheduled while that one's last blocks still run.
+// Launches a kernel that first of all waits (griddepcontrol.wait) for the launch
+// before it on `stream`: its blocks are scheduled while that one's last blocks
+// still run. All paged kernels are launched this way. `cluster` blocks form a
+// cluster where it is not 0.
 template <typename... Params, typename... Args>
-int launch_after(void (*kernel)(Params...), const char* name, dim3 grid, int threads,
-                 cudaStream_t stream, const Args&... args) {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+int launch_after(void (*kernel)(Params...), const char* name, long long grid, int threads, int smem,
+                 int cluster, void* stream, const Args&... args) {
+  cudaLaunchAttribute attr[2] = {};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(threads);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
   (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
   return launch_status(name);
 }
 
 template <int D>
 int append_launch(const AppendArgs& a, long long rows, int sms, void* stream) {
-  auto s = static_cast<cudaStream_t>(stream);
   const long long per = 256 / (D / 8);   // rows of a block, one a thread
   if (rows < 16 * per * sms)
-    append_kernel<D, 1><<<static_cast<unsigned>((rows + per - 1) / per), 256, 0, s>>>(a);
-  else
-    append_kernel<D, 4><<<static_cast<unsigned>((rows + 4 * per - 1) / (4 * per)), 256, 0, s>>>(a);
-  return launch_status("append_kernel");
+    return launch_after(append_kernel<D, 1>, "append_kernel", (rows + per - 1) / per, 256, 0, 0, stream, a);
+  return launch_after(append_kernel<D, 4>, "append_kernel", (rows + 4 * per - 1) / (4 * per), 256, 0, 0,
+                      stream, a);
 }
 
 // Threads of a one-block launch with `work` independent items.
@@ -292,7 +296,7 @@ int paged_cluster(long long units, long long most, int sms) {
 }
 
 template <int D, bool BF, int ROWS>
-int paged_attn_launch(PagedAttnArgs& a, int sms, cudaStream_t stream) {
+int paged_attn_launch(PagedAttnArgs& a, int sms, void* stream) {
   using C = PagedCfg<D>;
   const int group = a.Hq / a.Hkv;
   a.row_tiles = (group + ROWS - 1) / ROWS;
@@ -300,28 +304,17 @@ int paged_attn_launch(PagedAttnArgs& a, int sms, cudaStream_t stream) {
   a.step_rest = C::STEP % a.page;
   const long long units = static_cast<long long>(a.B) * a.Hkv * a.row_tiles;
   const long long most = (a.W * a.page + C::STEP - 1) / C::STEP;
-  if (const int c = paged_cluster(units, most, sms)) {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = c;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(units * c));
-    cfg.blockDim = dim3(128);
-    cfg.dynamicSmemBytes = C::SMEM;
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    (void)cudaLaunchKernelEx(&cfg, paged_attn_kernel<D, BF, ROWS, true>, a);
-    return launch_status("paged_attn_kernel (clusters)");
-  }
+  if (const int c = paged_cluster(units, most, sms))
+    return launch_after(paged_attn_kernel<D, BF, ROWS, true>, "paged_attn_kernel", units * c, 128, C::SMEM,
+                        c, stream, a);
   // two blocks an SM, fewer where the table has no room for so many steps
   const int blocks = static_cast<int>(std::min<double>(std::min(2 * sms, kPagedMaxBlocks),
                                                        static_cast<double>(units) * most));
-  paged_attn_kernel<D, BF, ROWS, false><<<blocks, 128, C::SMEM, stream>>>(a);
-  if (int st = launch_status("paged_attn_kernel")) return st;
-  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel", dim3(blocks), kJoinThreads,
-                      stream, a, ROWS);
+  if (int st = launch_after(paged_attn_kernel<D, BF, ROWS, false>, "paged_attn_kernel", blocks, 128, C::SMEM,
+                            0, stream, a))
+    return st;
+  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel", blocks, kJoinThreads, 0, 0, stream, a,
+                      ROWS);
 }
 
 template <int D, bool BF>
@@ -333,10 +326,9 @@ int paged_attn_impl(PagedAttnArgs& a, void* workspace, void* stream) {
   a.split = static_cast<int4*>(workspace);
   a.part_o = reinterpret_cast<float*>(a.split + kPagedMaxBlocks);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
-  auto s = static_cast<cudaStream_t>(stream);
-  if (group <= 8) return paged_attn_launch<D, BF, 8>(a, sms, s);
-  if (group <= 16) return paged_attn_launch<D, BF, 16>(a, sms, s);
-  return paged_attn_launch<D, BF, 32>(a, sms, s);
+  if (group <= 8) return paged_attn_launch<D, BF, 8>(a, sms, stream);
+  if (group <= 16) return paged_attn_launch<D, BF, 16>(a, sms, stream);
+  return paged_attn_launch<D, BF, 32>(a, sms, stream);
 }
 
 // An fp32 dQ is produced by the fused kernel: one pass, dQ added into the
@@ -992,15 +984,15 @@ int fa_b200_paged_extend(const int* new_lens, const int* lens, int* block_table,
   const fab::ExtendArgs a{new_lens, lens, free_pages, free_count, block_table, slots, granted,
                           lens_out, free_count_out, table_stride, head,
                           reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size, T};
-  auto s = static_cast<cudaStream_t>(stream);
   const bool wide = T > fab::kExtendWide;
-  fab::extend_kernel<<<1, fab::table_threads(std::max(B, T / fab::kSlotRun)), 0, s>>>(a, !wide);
-  if (int st = fab::launch_status("extend_kernel")) return st;
-  if (!wide) return FA_B200_OK;
   const long long runs = (T + fab::kSlotRun - 1ll) / fab::kSlotRun;
+  if (int st = fab::launch_after(fab::extend_kernel, "extend_kernel", 1,
+                                 fab::table_threads(wide ? B : std::max<long long>(B, runs)), 0, 0, stream,
+                                 a, !wide))
+    return st;
+  if (!wide) return FA_B200_OK;
   return fab::launch_after(fab::extend_fill_kernel, "extend_fill_kernel",
-                           dim3(static_cast<unsigned>(std::min<long long>((runs + 255) / 256, 8 * sms))),
-                           256, s, a);
+                           std::min<long long>((runs + 255) / 256, 8 * sms), 256, 0, 0, stream, a);
 }
 
 int fa_b200_paged_release(const unsigned char* finished, const int* lens, const int* block_table,
@@ -1023,15 +1015,15 @@ int fa_b200_paged_release(const unsigned char* finished, const int* lens, const 
   const fab::ReleaseArgs a{finished, lens, block_table, free_count, free_pages, lens_out,
                            free_count_out, table_stride, head,
                            reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size};
-  auto s = static_cast<cudaStream_t>(stream);
   const long long runs = static_cast<long long>(B) * ((W + fab::kReleaseRun - 1) / fab::kReleaseRun);
   const bool wide = std::min<long long>(P, static_cast<long long>(B) * W) > fab::kReleaseWide;
-  fab::release_kernel<<<1, fab::table_threads(std::max<long long>(B, wide ? 0 : 32 * runs)), 0, s>>>(a, !wide);
-  if (int st = fab::launch_status("release_kernel")) return st;
+  if (int st = fab::launch_after(fab::release_kernel, "release_kernel", 1,
+                                 fab::table_threads(wide ? B : std::max<long long>(B, 32 * runs)), 0, 0,
+                                 stream, a, !wide))
+    return st;
   if (!wide) return FA_B200_OK;
   return fab::launch_after(fab::release_fill_kernel, "release_fill_kernel",
-                           dim3(static_cast<unsigned>(std::min<long long>((runs + 7) / 8, 8 * sms))), 256,
-                           s, a);
+                           std::min<long long>((runs + 7) / 8, 8 * sms), 256, 0, 0, stream, a);
 }
 
 int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b200_strides sv,

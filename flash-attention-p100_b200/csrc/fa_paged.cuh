@@ -250,6 +250,7 @@ __device__ __forceinline__ void extend_fill_block(const ExtendArgs& a, long long
 }
 
 __global__ void __launch_bounds__(kTableThreads) extend_kernel(const ExtendArgs a, int fill) {
+  wait_for_prior_launch();
   const bool longer = extend_rows(a);
   if (!fill || !longer) return;
   __syncthreads();
@@ -322,6 +323,7 @@ __device__ __forceinline__ void release_fill(const ReleaseArgs& a, long long fir
 }
 
 __global__ void __launch_bounds__(kTableThreads) release_kernel(const ReleaseArgs a, int fill) {
+  wait_for_prior_launch();
   release_rows(a);
   if (!fill) return;
   __syncthreads();
@@ -348,6 +350,7 @@ struct AppendArgs {
 // loads ahead of the stores: 4 rows where that still fills the GPU, else 1. The pieces of a row are neighbouring threads.
 template <int D, int kAppendRows>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+  wait_for_prior_launch();
   constexpr int CH = D / 8, RPB = 256 / CH;   // pieces of a row, rows a block covers at once
   const long long rows = static_cast<long long>(a.T) * a.Hkv;
   const int c = static_cast<int>(threadIdx.x) % CH * 8;
@@ -621,6 +624,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
   const int cap = a.W * a.page;
+  wait_for_prior_launch();
   const auto length = [&](int b) { return min(max(a.lens[b], 0), cap); };
   const auto steps = [&](int len) { return (len + C::STEP - 1) / C::STEP; };
   const auto empty_row = [&](int b, int head0, int heads) {

@@ -300,8 +300,6 @@ int paged_attn_launch(PagedAttnArgs& a, int sms, void* stream) {
   using C = PagedCfg<D>;
   const int group = a.Hq / a.Hkv;
   a.row_tiles = (group + ROWS - 1) / ROWS;
-  a.step_pages = C::STEP / a.page;
-  a.step_rest = C::STEP % a.page;
   const long long units = static_cast<long long>(a.B) * a.Hkv * a.row_tiles;
   const long long most = (a.W * a.page + C::STEP - 1) / C::STEP;
   if (const int c = paged_cluster(units, most, sms))

@@ -420,7 +420,6 @@ struct PagedAttnArgs {
   long long table_stride;
   int B, Hq, Hkv, P, W, page;
   int row_tiles;              // tiles of ROWS heads in a group
-  int step_pages, step_rest;  // STEP = step_pages * page + step_rest
   float scale;     // log2(e) / sqrt(D)
   int4* split;     // per block: the unit whose first part it holds (b, kv head, row tile, last block), x < 0: none
   float2* part_ml; // per block two partial results: [2 block + first][row] max and sum
@@ -438,8 +437,8 @@ struct PagedCfg {
   static constexpr int ALL = GROUPS == 2 ? 0x1010 : 0x10;  // keys of the runs, 8 bits each, when all are real
   static constexpr int TILE = KEYS * D * 2;   // bytes of a warp's K (or V) of a step
   static constexpr int RING = WARPS * STAGES * 2 * TILE;
-  static constexpr int MERGE = 16 * D * 4;    // one warp's fp32 result of 16 rows
-  static constexpr int SMEM = RING + 2 * MERGE;
+  static constexpr int MERGE = WARPS * 8 * D * 4;  // the warps' fp32 results of 8 rows
+  static constexpr int SMEM = RING + MERGE;
 };
 
 constexpr int kPagedMaxBlocks = 320;  // blocks of a line at most: sizes the workspace
@@ -544,56 +543,38 @@ __device__ __forceinline__ void store_part_sum(const PagedAttnArgs& a, const Par
     a.lse[static_cast<long long>(b) * a.Hq + head] = 0.6931471805599453f * (x.m - weight_bias<BF>() + log2f(x.l));
 }
 
-// Adds the warps' results of a unit into warp 0's registers, fragment by fragment
-// (warps 2 and 3 hand theirs to 0 and 1, then 1 to 0), and calls done(fragment) in
-// warp 0. `buf` holds two fragments. Ends with other warps ahead of warp 0.
-template <typename C, int E, int MT, int N, typename Done>
-__device__ __forceinline__ void merge_warps(unsigned char* buf, float2 (&s_ml)[C::WARPS][16], float (&o)[MT][N][4],
-                                            float (&m)[MT][E], float (&l)[MT][E], const Done& done) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+// Adds up the warps' results of a unit, 8 rows at a time through shared memory
+// (`buf`, 8 D floats a warp; 32-byte pieces xor-ed with the row, so neither side
+// conflicts), and calls emit(row, column, sum) for every four columns.
+template <int D, int E, int MT, typename Emit>
+__device__ __forceinline__ void merge_warps(unsigned char* buf, float2 (&s_ml)[4][8], float (&o)[MT][D / 8][4],
+                                            float (&m)[MT][E], float (&l)[MT][E], const Emit& emit) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row_w = lane >> 2;
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
-      l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
-    }
-#pragma unroll
-    for (int half = C::WARPS / 2; half >= 1; half >>= 1) {
+      float sum = l[mt][e];
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
       __syncthreads();   // buf and s_ml are free
-      if (warp >= half && warp < 2 * half) {
-        float2* mine = reinterpret_cast<float2*>(buf + (warp - half) * C::MERGE);
+      unsigned char* mine = buf + (warp * 8 + row_w) * (D * 4) + (lane & 3) * 8;
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            mine[(i * E + e) * 32 + lane] = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if ((lane & 3) == 0) s_ml[warp][lane / 4 + 8 * e] = make_float2(m[mt][e], l[mt][e]);
-      }
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<float2*>(mine + ((i ^ row_w) << 5)) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+      if ((lane & 3) == 0) s_ml[warp][row_w] = make_float2(m[mt][e], sum);
       __syncthreads();
-      if (warp < half) {
-        const float2* other = reinterpret_cast<const float2*>(buf + warp * C::MERGE);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float2 x = s_ml[warp + half][lane / 4 + 8 * e];
-          const float mn = fmaxf(m[mt][e], x.x);
-          const float w = mn == -INFINITY ? 1.f : ex2(m[mt][e] - mn);
-          const float y = mn == -INFINITY ? 1.f : ex2(x.x - mn);
-          m[mt][e] = mn;
-          l[mt][e] = l[mt][e] * w + x.y * y;
+      for (int i = 0; i < 8 * (D / 4) / 128; ++i) {
+        const int at = i * 128 + static_cast<int>(threadIdx.x), row = at / (D / 4), col = at % (D / 4) * 4;
+        PartSum part;
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float2 z = other[(i * E + e) * 32 + lane];
-            o[mt][i][2 * e] = o[mt][i][2 * e] * w + z.x * y;
-            o[mt][i][2 * e + 1] = o[mt][i][2 * e + 1] * w + z.y * y;
-          }
-        }
+        for (int w = 0; w < 4; ++w)
+          part.add(s_ml[w][row], *reinterpret_cast<const float4*>(buf + (w * 8 + row) * (D * 4) +
+                                                                 (((col >> 3) ^ row) << 5) + (col & 4) * 4));
+        emit(mt * 16 + e * 8 + row, col, part);
       }
     }
-    if (warp == 0) done(mt);
-  }
 }
 
 __device__ __forceinline__ const uint4* unit_at(const uint4* base, const Units& s, uint32_t b, uint32_t h,
@@ -619,7 +600,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ long long s_sum[C::WARPS], s_at;
   __shared__ int s_b, s_valid[C::WARPS][C::STAGES];
-  __shared__ float2 s_ml[C::WARPS][16];
+  __shared__ float2 s_ml[C::WARPS][8];
   __shared__ float2 s_unit_ml[ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
@@ -637,7 +618,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   // ---- this block's steps ----
   PagedAt at;
   long long n_steps, total = 0, g1 = 0;
-  int blocks = 0, rank = 0, ranks = 1;
+  int blocks = 0, rank = 0, ranks = 1;   // ranks: also how many steps on the block's next one is
   if constexpr (CLUSTER) {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -646,14 +627,9 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     at.head = (unit - at.b * units) / a.row_tiles;
     at.rt = unit % a.row_tiles;
     at.len = length(at.b);
-    if (at.len == 0) {   // the whole cluster
-      const int head0 = at.head * group + at.rt * ROWS;
-      if (rank == 0) empty_row(at.b, head0, min(ROWS, group - at.rt * ROWS));
-      return;
-    }
     at.nt = steps(at.len);
-    at.t = static_cast<int>(static_cast<long long>(at.nt) * rank / ranks);
-    n_steps = static_cast<int>(static_cast<long long>(at.nt) * (rank + 1) / ranks) - at.t;
+    at.t = rank;     // steps in turn: where a block begins does not depend on the length
+    n_steps = at.nt > rank ? (at.nt - rank + ranks - 1) / ranks : 0;
   } else {
     // every block adds up the lengths itself; [g0, g1) is its stretch of the line
     const int per = (a.B + 127) / 128;
@@ -720,6 +696,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   // xor changes by a constant
   const uint32_t ring_lane = ring + lr * (D * 2) + ((lc ^ lr) << 4);
   const int key_w = warp * C::KEYS, page_w = key_w / a.page, off_w = key_w - page_w * a.page;
+  const int step_pages = ranks * C::STEP / a.page, step_rest = ranks * C::STEP - step_pages * a.page;
   // The next step to load and the one behind it, their pages already looked up.
   struct Next {
     PagedAt at;
@@ -727,17 +704,19 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     int ids[C::GROUPS];
   } ld, ld2;
   const auto fetch_ids = [&](Next& x) {
+    // entries behind the request's last page are not used, but in the table
     const int* row = a.table + x.at.b * a.table_stride;
 #pragma unroll
     for (int g = 0; g < C::GROUPS; ++g) {
-      const int past = x.off + g * 16 >= a.page;   // a page holds 16 or more
-      x.ids[g] = x.at.t * C::STEP + key_w + g * 16 < x.at.len ? row[x.page + past] : 0;
+      const int page = x.page + (x.off + g * 16 >= a.page);   // a page holds 16 or more
+      x.ids[g] = page < a.W ? row[page] : 0;
     }
   };
   const auto advance = [&](Next& x) {
-    if (++x.at.t < x.at.nt) {
-      x.page += a.step_pages;
-      x.off += a.step_rest;
+    x.at.t += ranks;
+    if (CLUSTER || x.at.t < x.at.nt) {
+      x.page += step_pages;
+      x.off += step_rest;
       if (x.off >= a.page) {
         x.off -= a.page;
         ++x.page;
@@ -787,13 +766,13 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   long long issued = 0;
   ld.at = at;
   {
-    const long long key = static_cast<long long>(at.t) * C::STEP + key_w;
-    ld.page = static_cast<int>(key / a.page);
-    ld.off = static_cast<int>(key - static_cast<long long>(ld.page) * a.page);
+    const int key = at.t * C::STEP + key_w;
+    ld.page = key / a.page;
+    ld.off = key - ld.page * a.page;
   }
-  if (n_steps > 0) fetch_ids(ld);
+  fetch_ids(ld);
   ld2 = ld;
-  if (n_steps > 1) {
+  if (CLUSTER || n_steps > 1) {
     advance(ld2);
     fetch_ids(ld2);
   }
@@ -808,9 +787,6 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     }
     cp_async_commit();
   };
-#pragma unroll
-  for (int s = 0; s < C::STAGES - 1; ++s) issue_next(s);
-
   // ---- per unit state ----
   uint32_t qf[MT][D / 16][4];
   float o[MT][D / 8][4], m[MT][E], l[MT][E];
@@ -850,6 +826,14 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   int first_t = at.t;
   load_q(at);
   clear();
+  if constexpr (CLUSTER) {
+    if (at.len == 0) {   // the whole cluster
+      if (rank == 0) empty_row(at.b, at.head * group + at.rt * ROWS, min(ROWS, group - at.rt * ROWS));
+      return;
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) issue_next(s);
   int stage = C::STAGES - 1;
   for (long long it = 0; it < n_steps; ++it) {
     const int free_stage = stage;
@@ -949,7 +933,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
         }
     }
     if (it + 1 < n_steps && (CLUSTER || at.t + 1 < at.nt)) {
-      ++at.t;
+      at.t += ranks;
       continue;
     }
     if constexpr (CLUSTER) break;
@@ -961,30 +945,15 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
       load_q(at);
     }
     const bool whole = first_t == 0 && done.t + 1 == done.nt;
-    merge_warps<C, E, MT>(smem + C::RING, s_ml, o, m, l, [&](int mt) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int row = mt * 16 + e * 8 + lane / 4, r = done.rt * ROWS + row;
-        if (r >= group) continue;
-        const int head = done.head * group + r;
-        if (whole) {
-          const float inv = 1.f / l[mt][e];
-          uint16_t* out = a.o + a.so.at(done.b, head, 0) + (lane & 3) * 2;
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-            *reinterpret_cast<uint32_t*>(out + i * 8) =
-                pack16<BF>(o[mt][i][2 * e] * inv, o[mt][i][2 * e + 1] * inv);
-          if ((lane & 3) == 0)
-            a.lse[static_cast<long long>(done.b) * a.Hq + head] =
-                0.6931471805599453f * (m[mt][e] - kBias + log2f(l[mt][e]));
-        } else {
-          const long long slot = (2ll * blockIdx.x + (first_t == 0)) * min(group, ROWS) + row;
-          float* out = a.part_o + slot * D + (lane & 3) * 2;
-#pragma unroll
-          for (int i = 0; i < D / 8; ++i)
-            *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
-          if ((lane & 3) == 0) a.part_ml[slot] = make_float2(m[mt][e], l[mt][e]);
-        }
+    merge_warps<D, E, MT>(smem + C::RING, s_ml, o, m, l, [&](int row, int col, const PartSum& x) {
+      const int r = done.rt * ROWS + row;
+      if (r >= group) return;
+      if (whole) {
+        store_part_sum<BF>(a, x, done.b, done.head * group + r, col);
+      } else {
+        const long long slot = (2ll * blockIdx.x + (first_t == 0)) * min(group, ROWS) + row;
+        *reinterpret_cast<float4*>(a.part_o + slot * D + col) = x.o;
+        if (col == 0) a.part_ml[slot] = make_float2(x.m, x.l);
       }
     });
     if (!whole && first_t == 0 && threadIdx.x == 0) {
@@ -1001,16 +970,9 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     // this block's part into its shared memory (the ring: every load has landed
     // and been read), then every block adds up a share of the columns
     float* part = reinterpret_cast<float*>(smem);
-    merge_warps<C, E, MT>(smem + C::RING, s_ml, o, m, l, [&](int mt) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int row = mt * 16 + e * 8 + lane / 4;
-        float* out = part + row * D + (lane & 3) * 2;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<float2*>(out + i * 8) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
-        if ((lane & 3) == 0) s_unit_ml[row] = make_float2(m[mt][e], l[mt][e]);
-      }
+    merge_warps<D, E, MT>(smem + C::RING, s_ml, o, m, l, [&](int row, int col, const PartSum& x) {
+      *reinterpret_cast<float4*>(part + row * D + col) = x.o;
+      if (col == 0) s_unit_ml[row] = make_float2(x.m, x.l);
     });
     cluster_sync();
     const int rows = min(ROWS, group - at.rt * ROWS), head0 = at.head * group + at.rt * ROWS;

@@ -235,7 +235,7 @@ int launch_status(const char* kernel) {
 // still run. All paged kernels are launched this way. `cluster` blocks form a
 // cluster where it is not 0.
 template <typename... Params, typename... Args>
-int launch_after(void (*kernel)(Params...), const char* name, long long grid, int threads, int smem,
+int launch_after(void (*kernel)(Params...), const char* name, dim3 grid, int threads, int smem,
                  int cluster, void* stream, const Args&... args) {
   cudaLaunchAttribute attr[2] = {};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -244,7 +244,7 @@ int launch_after(void (*kernel)(Params...), const char* name, long long grid, in
   attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
@@ -311,8 +311,13 @@ int paged_attn_launch(PagedAttnArgs& a, int sms, void* stream) {
   if (int st = launch_after(paged_attn_kernel<D, BF, ROWS, false>, "paged_attn_kernel", blocks, 128, C::SMEM,
                             0, stream, a))
     return st;
-  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel", blocks, kJoinThreads, 0, 0, stream, a,
-                      ROWS);
+  // few units: many parts each, so 16 columns a block and 16 threads for each of them
+  const int most_cols = 8 * units <= blocks ? 16 : kJoinThreads;
+  const int cols = std::min(group, ROWS) * (D / 4);
+  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel",
+                      dim3(static_cast<unsigned>(std::min<long long>(units, blocks)),
+                           (cols + most_cols - 1) / most_cols),
+                      kJoinThreads, 0, 0, stream, a, ROWS, most_cols);
 }
 
 template <int D, bool BF>
@@ -1070,6 +1075,7 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
   if (table_stride < W) return FA_B200_ERR_SHAPE;
   if (int st = fab::check_pages(P, W, page_size)) return st;
   if (dtype != FA_B200_DTYPE_FP16 && dtype != FA_B200_DTYPE_BF16) return FA_B200_ERR_DTYPE;
+  if (static_cast<long long>(B) * Hq > 0x7fffffffll) return FA_B200_ERR_TOO_LARGE;
   if (!workspace || workspace_bytes < fab::paged_workspace(Hq / Hkv, D)) return FA_B200_ERR_WORKSPACE;
   fab::PagedAttnArgs a{};
   a.q = static_cast<const uint16_t*>(q);

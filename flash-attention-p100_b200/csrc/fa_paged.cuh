@@ -421,7 +421,10 @@ struct PagedAttnArgs {
   int B, Hq, Hkv, P, W, page;
   int row_tiles;              // tiles of ROWS heads in a group
   float scale;     // log2(e) / sqrt(D)
-  int4* split;     // per block: the unit whose first part it holds (b, kv head, row tile, last block), x < 0: none
+  // What paged_join_kernel has to add up: {unit, first block, last block}, unit < 0
+  // for nothing. One per unit where there are no more units than blocks, else one
+  // per block, of the unit that begins and does not end in it.
+  int4* split;
   float2* part_ml; // per block two partial results: [2 block + first][row] max and sum
   float* part_o;   // ... and [2 block + first][row][D]
   int* err;
@@ -605,6 +608,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
   const int cap = a.W * a.page;
+  const bool by_unit = static_cast<long long>(a.B) * units <= gridDim.x;
   wait_for_prior_launch();
   const auto length = [&](int b) { return min(max(a.lens[b], 0), cap); };
   const auto steps = [&](int len) { return (len + C::STEP - 1) / C::STEP; };
@@ -665,9 +669,13 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
       s_b = b;
       s_at = g0 - first;
     }
-    if (threadIdx.x == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-      if (length(b) == 0) empty_row(b, 0, a.Hq);
+    if (!by_unit && threadIdx.x == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      if (length(b) != 0) continue;
+      empty_row(b, 0, a.Hq);
+      if (by_unit)
+        for (int u = threadIdx.x; u < units; u += 128) a.split[b * units + u] = make_int4(-1, 0, 0, 0);
+    }
     __syncthreads();
     if (n_steps == 0) return;
     at.b = s_b;
@@ -956,11 +964,11 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
         if (col == 0) a.part_ml[slot] = make_float2(x.m, x.l);
       }
     });
-    if (!whole && first_t == 0 && threadIdx.x == 0) {
-      // the block that holds the unit's last step
-      const long long last = g1 - 1 + (done.nt - 1 - done.t);
-      a.split[blockIdx.x] = make_int4(done.b, done.head, done.rt,
-                                      static_cast<int>(((last + 1) * blocks - 1) / total));
+    if (first_t == 0 && threadIdx.x == 0 && (by_unit || !whole)) {
+      const int unit = (done.b * a.Hkv + done.head) * a.row_tiles + done.rt;
+      const long long last = g1 - 1 + (done.nt - 1 - done.t);   // the unit's last step, where it is cut
+      a.split[by_unit ? unit : static_cast<int>(blockIdx.x)] =
+          make_int4(whole ? -1 : unit, blockIdx.x, whole ? 0 : static_cast<int>(((last + 1) * blocks - 1) / total), 0);
     }
     first_t = 0;
     clear();
@@ -1000,26 +1008,28 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
 }
 
 // Adds the parts of the units that a border of paged_attn_kernel cut: block x
-// takes the unit whose first part block x of that launch holds. The parts are
-// those of consecutive blocks, so in key order. A thread owns four columns of a
-// row and up to every fourth part, four of them in flight with a running
+// takes record x, and blocks y the unit's columns in turn, `most` at a time. The
+// parts are those of consecutive blocks, so in key order. A thread owns four
+// columns of a row and some of the parts, four of them in flight with a running
 // maximum; the threads of a column meet in shared memory.
 constexpr int kJoinThreads = 256;
 
 template <int D, bool BF>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int row_tile) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int row_tile, int most) {
   __shared__ float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
   wait_for_prior_launch();
-  const int4 unit = a.split[blockIdx.x];
-  if (unit.x < 0) return;
+  const int4 record = a.split[blockIdx.x];
+  if (record.x < 0) return;
   const int group = a.Hq / a.Hkv, rows = min(group, row_tile);
-  const int n = unit.w - static_cast<int>(blockIdx.x) + 1;
-  const int cols = min(rows, group - unit.z * row_tile) * (D / 4);
+  const int rt = record.x % a.row_tiles, b = record.x / (a.row_tiles * a.Hkv);
+  const int head0 = (record.x / a.row_tiles - b * a.Hkv) * group + rt * row_tile;
+  const int first = record.y, n = record.z - record.y + 1;
+  const int cols = min(rows, group - rt * row_tile) * (D / 4);
   // as many threads a column as give each up to four parts
-  const int width = min(cols, kJoinThreads), parts = min(kJoinThreads / width, (n + 3) / 4);
+  const int width = min(cols, most), parts = min(kJoinThreads / width, (n + 3) / 4);
   const int part = static_cast<int>(threadIdx.x) / width;
-  for (int c0 = 0; c0 < cols; c0 += width) {
+  for (int c0 = blockIdx.y * width; c0 < cols; c0 += gridDim.y * width) {
     const int c = c0 + static_cast<int>(threadIdx.x) % width, r = c / (D / 4), col = c % (D / 4) * 4;
     const bool mine = part < parts && c < cols;
     PartSum sum;
@@ -1031,7 +1041,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int i = min(i0 + j * parts, n - 1);
-          const long long slot = (2ll * (blockIdx.x + i) + (i == 0)) * rows + r;
+          const long long slot = (2ll * (first + i) + (i == 0)) * rows + r;
           ml[j] = a.part_ml[slot];
           x[j] = *reinterpret_cast<const float4*>(a.part_o + slot * D + col);
         }
@@ -1045,7 +1055,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
     __syncthreads();
     if (mine && part == 0) {
       for (int p = 1; p < parts; ++p) sum.add(s_ml[p * width + threadIdx.x], s_o[p * width + threadIdx.x]);
-      store_part_sum<BF>(a, sum, unit.x, unit.y * group + unit.z * row_tile + r, col);
+      store_part_sum<BF>(a, sum, b, head0 + r, col);
     }
     __syncthreads();
   }

@@ -546,6 +546,23 @@ __device__ __forceinline__ void store_part_sum(const PagedAttnArgs& a, const Par
     a.lse[static_cast<long long>(b) * a.Hq + head] = 0.6931471805599453f * (x.m - weight_bias<BF>() + log2f(x.l));
 }
 
+// x + y, the sums of the weights' first and second terms; x alone where it is not
+// finite: an infinite value times a second term of 0 or below says nothing.
+__device__ __forceinline__ float add_finite(float x, float y) { return fabsf(x) < INFINITY ? x + y : x; }
+
+// Two 16-bit values, infinities (and NaN) replaced by finite ones, for the same reason.
+template <bool BF>
+__device__ __forceinline__ uint32_t finite16(uint32_t x) {
+  if (BF) {
+    const __nv_bfloat162 top = __nv_bfloat162(__ushort_as_bfloat16(0x7f7f), __ushort_as_bfloat16(0x7f7f));
+    const __nv_bfloat162 y = __hmin2(__hmax2(*reinterpret_cast<const __nv_bfloat162*>(&x), __hneg2(top)), top);
+    return *reinterpret_cast<const uint32_t*>(&y);
+  }
+  const __half2 top = __half2(__ushort_as_half(0x7bff), __ushort_as_half(0x7bff));
+  const __half2 y = __hmin2(__hmax2(*reinterpret_cast<const __half2*>(&x), __hneg2(top)), top);
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
 // Adds up the warps' results of a unit, 8 rows at a time through shared memory
 // (`buf`, 8 D floats a warp; 32-byte pieces xor-ed with the row, so neither side
 // conflicts), and calls emit(row, column, sum) for every four columns.
@@ -564,7 +581,9 @@ __device__ __forceinline__ void merge_warps(unsigned char* buf, float2 (&s_ml)[4
       unsigned char* mine = buf + (warp * 8 + row_w) * (D * 4) + (lane & 3) * 8;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
-        *reinterpret_cast<float2*>(mine + ((i ^ row_w) << 5)) = make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
+        *reinterpret_cast<float2*>(mine + ((i ^ row_w) << 5)) =
+            E == 1 ? make_float2(add_finite(o[mt][i][0], o[mt][i][2]), add_finite(o[mt][i][1], o[mt][i][3]))
+                   : make_float2(o[mt][i][2 * e], o[mt][i][2 * e + 1]);
       if ((lane & 3) == 0) s_ml[warp][row_w] = make_float2(m[mt][e], sum);
       __syncthreads();
 #pragma unroll
@@ -592,8 +611,8 @@ struct PagedAt {
   int len;
 };
 
-// ROWS query heads of a group per unit: 8 (the lower half of an m16 fragment,
-// half the softmax), 16 (one fragment) or 32 (two); a group above 32 is cut into
+// ROWS query heads of a group per unit: 8 (half of an m16 fragment, whose other
+// half takes the weights' second terms), 16 (one fragment) or 32 (two); a group above 32 is cut into
 // row tiles, each of which reads the cache again.
 template <int D, bool BF, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) {
@@ -883,7 +902,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
               if (key + (e & 1) >= n) s[mt][i][e] = -INFINITY;
         }
       }
-      uint32_t p[MT][C::GROUPS][4];
+      uint32_t p[MT][C::GROUPS][4], p2[MT][C::GROUPS][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         float top[E];
@@ -899,7 +918,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
           grown |= top[e] > m[mt][e] + 8.f;
         }
         if (__any_sync(0xffffffffu, grown)) {
-          float w[2] = {1.f, 1.f};
+          float w[E];
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             const float mn = fmaxf(m[mt][e], top[e]);
@@ -910,20 +929,29 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
 #pragma unroll
           for (int i = 0; i < D / 8; ++i)
 #pragma unroll
-            for (int e = 0; e < 2 * E; ++e) o[mt][i][e] *= w[e >> 1];
+            for (int e = 0; e < 4; ++e) o[mt][i][e] *= w[E == 1 ? 0 : e >> 1];
         }
+        // Weights enter the product with v as two 16-bit terms, the rounded weight
+        // and what the rounding left, so that neither o nor (summed in fp32) lse
+        // loses to it. The second terms of 8 rows are the fragment's other 8.
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const float ref = m[mt][e] == -INFINITY ? 0.f : kBias - m[mt][e];
 #pragma unroll
           for (int i = 0; i < 2 * C::GROUPS; ++i) {
-            // the sum takes the weights as the product with v takes them: rounded
-            const uint32_t w = pack16<BF>(ex2(fmaf(s[mt][i][2 * e], a.scale, ref)),
-                                          ex2(fmaf(s[mt][i][2 * e + 1], a.scale, ref)));
-            const float2 r = unpack16<BF>(w);
-            l[mt][e] += r.x + r.y;
-            p[mt][i >> 1][2 * (i & 1) + e] = w;
-            if (E == 1) p[mt][i >> 1][2 * (i & 1) + 1] = 0;
+            const float x = ex2(fmaf(s[mt][i][2 * e], a.scale, ref));
+            const float y = ex2(fmaf(s[mt][i][2 * e + 1], a.scale, ref));
+            l[mt][e] += x + y;
+            const uint32_t hi = pack16<BF>(x, y);
+            const float2 r = unpack16<BF>(hi);
+            const uint32_t lo = pack16<BF>(x - r.x, y - r.y);
+            if (E == 1) {
+              p[mt][i >> 1][2 * (i & 1)] = hi;
+              p[mt][i >> 1][2 * (i & 1) + 1] = lo;
+            } else {
+              p[mt][i >> 1][2 * (i & 1) + e] = hi;
+              p2[mt][i >> 1][2 * (i & 1) + e] = lo;
+            }
           }
         }
       }
@@ -937,6 +965,15 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
           for (int mt = 0; mt < MT; ++mt) {
             mma16<BF>(o[mt][2 * dt], p[mt][g], f[0], f[1]);
             mma16<BF>(o[mt][2 * dt + 1], p[mt][g], f[2], f[3]);
+          }
+          if constexpr (E == 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = finite16<BF>(f[i]);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              mma16<BF>(o[mt][2 * dt], p2[mt][g], f[0], f[1]);
+              mma16<BF>(o[mt][2 * dt + 1], p2[mt][g], f[2], f[3]);
+            }
           }
         }
     }

@@ -13,7 +13,9 @@ Contract kept from the reference (fa_p100_hf.py:46-213):
   * everything the kernel cannot do raises NotImplementedError rather than
     degrading: attention masks, output_attentions, head_mask, sliding windows,
     dropout, head_dim outside {64, 128}, a scale other than 1/sqrt(D), and
-    q_len != kv_len (a populated KV cache);
+    q_len != kv_len (a populated KV cache) -- but for the paged cache of
+    make_cache (beyond the reference), whose decoding steps run through
+    fa_p100_paged;
   * fp16 inputs run as they are, and so (beyond the reference) do bf16 ones;
     other dtypes (or a mix) are cast to the autocast dtype under fp16 or bf16
     autocast, and to fp16 with a single warning outside autocast. Outside
@@ -33,8 +35,9 @@ _IMPL_NAME = "fa_p100"
 _warned_cast = False
 
 
-def _unsupported(attention_mask, dropout, scaling, query, key, kwargs):
-    """The first reason this call cannot be served, or None."""
+def _unsupported(attention_mask, dropout, scaling, query, key, kwargs, past=None):
+    """The first reason this call cannot be served, or None. `past`: tokens that the
+    paged cache held before this call's, None without one."""
     head_dim = query.size(-1)
     if attention_mask is not None:
         return ("fa_p100 got an attention mask, but the kernel takes none; pack "
@@ -54,6 +57,9 @@ def _unsupported(attention_mask, dropout, scaling, query, key, kwargs):
     if scaling is not None and abs(scaling - head_dim ** -0.5) > 1e-6:
         return (f"fa_p100 always scales by 1/sqrt(D) = {head_dim ** -0.5:.6g}; the "
                 f"model asks for {scaling:.6g}")
+    if past and query.size(2) > 1:
+        return (f"fa_p100 adds one token at a time to a cache that holds tokens ({past} here, "
+                f"{query.size(2)} new); reset the cache, or run the prompt in one call")
     if key.size(2) != query.size(2):
         return (f"fa_p100 needs equal query and key lengths, got q={query.size(2)} "
                 f"kv={key.size(2)}: that is KV-cache decoding, which this training "
@@ -65,9 +71,14 @@ def fa_p100_attention_forward(module, query, key, value, attention_mask, dropout
                               scaling=None, is_causal=None, **kwargs):
     """transformers attention-interface entry point (fa_p100_hf.py:46-142)."""
     global _warned_cast
-    reason = _unsupported(attention_mask, dropout, scaling, query, key, kwargs)
+    # the paged cache marks the keys it has just stored
+    layer, past = getattr(key, "_fa_p100_paged", (None, None))
+    reason = _unsupported(attention_mask, dropout, scaling, query, key, kwargs, past)
     if reason is not None:
         raise NotImplementedError(reason)
+    if past:
+        out = layer.attention(query)
+        return (out if torch.is_autocast_enabled("cuda") else out.to(query.dtype)), None
 
     if is_causal is None:
         is_causal = bool(getattr(module, "is_causal", True)) and query.size(2) > 1
@@ -129,7 +140,7 @@ def enable_fa_p100(model, full_precision=False):
             _set_impl(cfg, _IMPL_NAME)
         mod._fa_p100_full_precision = full_precision
 
-    # q_len == kv_len is required, so a KV cache can never be used: default it off.
+    # q_len == kv_len is required, so only make_cache's cache can be used: default it off.
     model.config.use_cache = False
     if getattr(model, "generation_config", None) is not None:
         model.generation_config.use_cache = False
@@ -145,12 +156,28 @@ def enable_fa_p100(model, full_precision=False):
                     "fa_p100 cannot apply a padding mask and transformers would drop "
                     "it without a word; pack the batch so every position is real")
             # Raised here, before prefill, not at the first decode step.
-            if use_cache:
+            if use_cache and not getattr(kwargs.get("past_key_values"), "_fa_p100_paged", False):
                 raise NotImplementedError(
-                    "fa_p100 needs q_len == kv_len and so cannot use a KV cache; for "
-                    "cache-free generation set generation_config.use_cache = False")
+                    "fa_p100 needs q_len == kv_len and so cannot use a KV cache other than "
+                    "make_cache's; for cache-free generation set "
+                    "generation_config.use_cache = False")
             return wrapped(*args, attention_mask=attention_mask, use_cache=use_cache, **kwargs)
 
         model.forward = guarded_forward
         model._fa_p100_guarded = True
     return model
+
+
+def make_cache(model, batch, max_len, page_size=64, dtype=None):
+    """A paged key-value cache for generation with `model` (after enable_fa_p100):
+    pass it as past_key_values together with use_cache=True. It holds up to max_len
+    tokens of each of `batch` sequences of one length, in fp16 or bf16 (default:
+    the model's dtype where it is one of these, else fp16, as outside autocast)."""
+    from fa_p100_hf_cache import FaP100Cache
+
+    cfg = model.config.get_text_config()
+    heads = getattr(cfg, "num_key_value_heads", None) or cfg.num_attention_heads
+    head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // cfg.num_attention_heads
+    if dtype is None:
+        dtype = model.dtype if model.dtype in (torch.float16, torch.bfloat16) else torch.float16
+    return FaP100Cache(cfg.num_hidden_layers, heads, head_dim, batch, max_len, page_size, dtype, model.device)

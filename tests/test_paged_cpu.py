@@ -202,3 +202,48 @@ def test_attn_argument_errors():
     assert c_attn(q=P + 1) == 4
     assert c_attn(sq=_lib.Strides(4 * 64 + 4, 64, 64)) == 4
     assert "page" in _lib.status_string(13)
+
+
+# ---- the HuggingFace cache ----
+def _model():
+    import fa_p100_hf
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+    cfg = Qwen3Config(vocab_size=64, hidden_size=128, intermediate_size=256, num_hidden_layers=2,
+                      num_attention_heads=2, num_key_value_heads=1, head_dim=64,
+                      max_position_embeddings=64, tie_word_embeddings=True)
+    return fa_p100_hf.enable_fa_p100(Qwen3ForCausalLM(cfg))
+
+
+def test_hf_cache_shape_and_guards():
+    import fa_p100_hf
+    model = _model()
+    cache = fa_p100_hf.make_cache(model, batch=3, max_len=100, page_size=32)
+    assert cache.paged.k.shape == (2, 12, 1, 32, 64) and cache.paged.k.dtype == torch.float16
+    assert len(cache.layers) == 2 and cache.get_seq_length() == 0 and cache.get_max_cache_shape() == 128
+    assert fa_p100_hf.make_cache(model.bfloat16(), 1, 10).paged.k.dtype == torch.bfloat16
+    ids = torch.zeros(3, 8, dtype=torch.long)
+    # the guard lets this cache through (the operators then refuse CPU tensors) and no other
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+        model(ids, past_key_values=cache, use_cache=True)
+    with pytest.raises(NotImplementedError, match="KV cache"):
+        model(ids, use_cache=True)
+    with pytest.raises(NotImplementedError, match="padding mask"):
+        model(ids, past_key_values=cache, use_cache=True, attention_mask=torch.tensor([[0] + [1] * 7] * 3))
+    with pytest.raises(NotImplementedError, match="in place"):
+        cache.reorder_cache(torch.tensor([0, 0, 1]))
+    with pytest.raises(RuntimeError, match="batch of 3"):
+        cache.update(torch.zeros(2, 1, 4, 64), torch.zeros(2, 1, 4, 64), 0)
+    with pytest.raises(RuntimeError, match="do not fit"):
+        cache.update(torch.zeros(3, 1, 129, 64), torch.zeros(3, 1, 129, 64), 0)
+
+
+def test_hf_attention_refuses_a_second_prompt():
+    import fa_p100_hf
+
+    class Layer:
+        is_causal = True
+
+    k = torch.zeros(1, 2, 8, 64, dtype=torch.float16)
+    k._fa_p100_paged = (None, 5)
+    with pytest.raises(NotImplementedError, match="one token at a time"):
+        fa_p100_hf.fa_p100_attention_forward(Layer(), torch.zeros(1, 4, 8, 64).half(), k, k, None)

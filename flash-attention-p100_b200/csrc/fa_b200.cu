@@ -254,15 +254,6 @@ int launch_after(void (*kernel)(Params...), const char* name, dim3 grid, int thr
   return launch_status(name);
 }
 
-template <int D>
-int append_launch(const AppendArgs& a, long long rows, int sms, void* stream) {
-  const long long per = 256 / (D / 8);   // rows of a block, one a thread
-  if (rows < 16 * per * sms)
-    return launch_after(append_kernel<D, 1>, "append_kernel", (rows + per - 1) / per, 256, 0, 0, stream, a);
-  return launch_after(append_kernel<D, 4>, "append_kernel", (rows + 4 * per - 1) / (4 * per), 256, 0, 0,
-                      stream, a);
-}
-
 // Threads of a one-block launch with `work` independent items.
 int table_threads(long long work) {
   return static_cast<int>(std::min<long long>(kTableThreads, std::max<long long>(128, (work + 31) / 32 * 32)));
@@ -284,14 +275,25 @@ bool to_units(const Strides& s, int P, int Hkv, Units* u) {
   return true;
 }
 
-// Blocks of a cluster for `units` units whose table rows hold up to `most` steps,
-// 0 where the line is used. Clusters of 16, 8 or 4 blocks that together
-// fill the SMs at most once (two blocks each) and take at most kClusterSteps
-// steps of a full row per block.
-constexpr int kClusterSteps = 8;
+// Blocks of a cluster for `units` units whose table rows hold up to `most` steps
+// (32 KB of cache each), 0 where the line is used. Clusters need all their blocks
+// at once: two blocks an SM, one for clusters of 16, which fill a GPC. The line
+// keeps every SM busy whatever the lengths, but adds them up first and joins in a
+// second launch. Device time of a call, clusters / line, in us (bf16):
+//   8 kv heads, D=128, 1 request:    512 tokens 4.6 / 7.1, 2048 6.7 / 7.8, 8192 12.3 / 10.7
+//   32 requests of 512 tokens 11.0 / 14.7, of 1 to 512 10.3 / 13.2, of 1 to 1024 16.2 / 18.5
+//   20 requests (160 blocks) of 512 tokens 10.7 / 12.7, of 1024 17.4 / 16.5
+//   40 requests (two blocks a unit, in waves) of 256 tokens 14.9 / 12.9
+//   1 kv head, D=64, 1 request: 2048 tokens 5.1 / 6.6, 8192 7.7 / 7.0, 16000 13.2 / 8.4
+// so the steps a block may have to take grow with the part of the GPU in use.
 int paged_cluster(long long units, long long most, int sms) {
-  for (int c = 16; c >= 4; c /= 2)
-    if (units * c <= 2 * sms) return most <= static_cast<long long>(c) * kClusterSteps ? c : 0;
+  for (int c = 16; c >= 1; c /= 2) {
+    const long long blocks = units * c;
+    if (c > 1 && c / 2 >= most) continue;   // no more blocks than steps
+    if (blocks > (c == 16 ? sms : 2 * sms)) continue;
+    const int steps = 2 * blocks > 3 * sms ? 16 : 2 * blocks > sms ? 8 : 4;
+    return most <= static_cast<long long>(c) * steps ? c : 0;
+  }
   return 0;
 }
 
@@ -311,6 +313,7 @@ int paged_attn_launch(PagedAttnArgs& a, int sms, void* stream) {
   if (int st = launch_after(paged_attn_kernel<D, BF, ROWS, false>, "paged_attn_kernel", blocks, 128, C::SMEM,
                             0, stream, a))
     return st;
+  if (most == 1) return FA_B200_OK;   // nothing is cut
   // few units: many parts each, so 16 columns a block and 16 threads for each of them
   const int most_cols = 8 * units <= blocks ? 16 : kJoinThreads;
   const int cols = std::min(group, ROWS) * (D / 4);
@@ -1019,7 +1022,7 @@ int fa_b200_paged_release(const unsigned char* finished, const int* lens, const 
                            free_count_out, table_stride, head,
                            reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size};
   const long long runs = static_cast<long long>(B) * ((W + fab::kReleaseRun - 1) / fab::kReleaseRun);
-  const bool wide = std::min<long long>(P, static_cast<long long>(B) * W) > fab::kReleaseWide;
+  const bool wide = runs > fab::kReleaseWide;
   if (int st = fab::launch_after(fab::release_kernel, "release_kernel", 1,
                                  fab::table_threads(wide ? B : std::max<long long>(B, 32 * runs)), 0, 0,
                                  stream, a, !wide))
@@ -1048,14 +1051,15 @@ int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b2
       !fab::aligned16(v_cache) || !fab::strides_ok(a.sk, 2) || !fab::strides_ok(a.sv, 2) ||
       !fab::strides_ok(a.skc, 2) || !fab::strides_ok(a.svc, 2))
     return FA_B200_ERR_ALIGNMENT;
-  const long long rows = static_cast<long long>(T) * Hkv;
-  if (rows > (0x7fffffffll << 4)) return FA_B200_ERR_TOO_LARGE;
+  const long long rows = static_cast<long long>(T) * Hkv, per_block = 256 / (D / 8);
+  const long long blocks = (rows + per_block - 1) / per_block;
+  if (blocks > 0x7fffffffll) return FA_B200_ERR_TOO_LARGE;
   if (T == 0) return FA_B200_OK;
-  int dev = 0, sms = 0;
+  int dev = 0;
   int* err = nullptr;
-  if (int st = fab::device_setup(&dev, &err, &sms)) return st;
-  return D == 64 ? fab::append_launch<64>(a, rows, sms, stream)
-                 : fab::append_launch<128>(a, rows, sms, stream);
+  if (int st = fab::device_setup(&dev, &err)) return st;
+  return fab::launch_after(D == 64 ? fab::append_kernel<64> : fab::append_kernel<128>, "append_kernel",
+                           static_cast<unsigned>(blocks), 256, 0, 0, stream, a);
 }
 
 size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size) {

@@ -25,8 +25,9 @@ namespace fab {
 // few, else by a second launch that fills the GPU and whose start overlaps the
 // first (kExtendWide, kReleaseWide).
 constexpr int kTableThreads = 1024;
-// Slots (extend) and table entries (release) above which the second launch pays.
-constexpr int kExtendWide = 8192, kReleaseWide = 65536;
+// Slots (extend), and runs of kReleaseRun table entries (release), above which the
+// second launch pays.
+constexpr int kExtendWide = 4096, kReleaseWide = 32;
 // Up to this many tokens a request's own thread writes them (a decoding step);
 // a page holds 16 or more, so they take at most one new page.
 constexpr int kSlotsByRow = 4;
@@ -346,35 +347,24 @@ struct AppendArgs {
   int T, Hkv, P, page;
 };
 
-// A 16-byte piece of k and of v of kAppendRows (token, head) rows per thread, all
-// loads ahead of the stores: 4 rows where that still fills the GPU, else 1. The pieces of a row are neighbouring threads.
-template <int D, int kAppendRows>
+// A 16-byte piece of k and of v per thread; the pieces of a row are neighbouring
+// threads. Bound by HBM: 65536 tokens of 8 heads of 128 take 81 us, 6.6 TB/s read
+// and written (several rows a thread are no faster there and slower below).
+template <int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   wait_for_prior_launch();
-  constexpr int CH = D / 8, RPB = 256 / CH;   // pieces of a row, rows a block covers at once
-  const long long rows = static_cast<long long>(a.T) * a.Hkv;
+  constexpr int CH = D / 8;
+  const long long row = static_cast<long long>(blockIdx.x) * (256 / CH) + threadIdx.x / CH;
+  if (row >= static_cast<long long>(a.T) * a.Hkv) return;
   const int c = static_cast<int>(threadIdx.x) % CH * 8;
-  const long long row0 = static_cast<long long>(blockIdx.x) * (RPB * kAppendRows) + threadIdx.x / CH;
-  uint4 k[kAppendRows], v[kAppendRows];
-  int slot[kAppendRows], head[kAppendRows];
-#pragma unroll
-  for (int i = 0; i < kAppendRows; ++i) {
-    const long long row = row0 + i * RPB;
-    slot[i] = -1;
-    if (row >= rows) continue;
-    const int t = static_cast<int>(row / a.Hkv);
-    head[i] = static_cast<int>(row - static_cast<long long>(t) * a.Hkv);
-    slot[i] = a.slots[t];
-    k[i] = *reinterpret_cast<const uint4*>(a.k + a.sk.at(0, head[i], t) + c);
-    v[i] = *reinterpret_cast<const uint4*>(a.v + a.sv.at(0, head[i], t) + c);
-  }
-#pragma unroll
-  for (int i = 0; i < kAppendRows; ++i) {
-    if (slot[i] < 0 || slot[i] >= a.P * a.page) continue;
-    const int id = slot[i] / a.page, off = slot[i] - id * a.page;
-    *reinterpret_cast<uint4*>(a.k_cache + a.skc.at(id, head[i], off) + c) = k[i];
-    *reinterpret_cast<uint4*>(a.v_cache + a.svc.at(id, head[i], off) + c) = v[i];
-  }
+  const int t = static_cast<int>(row / a.Hkv), h = static_cast<int>(row - static_cast<long long>(t) * a.Hkv);
+  const int slot = a.slots[t];
+  const uint4 k = *reinterpret_cast<const uint4*>(a.k + a.sk.at(0, h, t) + c);
+  const uint4 v = *reinterpret_cast<const uint4*>(a.v + a.sv.at(0, h, t) + c);
+  if (slot < 0 || slot >= a.P * a.page) return;
+  const int id = slot / a.page, off = slot - id * a.page;
+  *reinterpret_cast<uint4*>(a.k_cache + a.skc.at(id, h, off) + c) = k;
+  *reinterpret_cast<uint4*>(a.v_cache + a.svc.at(id, h, off) + c) = v;
 }
 
 // ---------------------------------------------------------------------------

@@ -259,13 +259,6 @@ int table_threads(long long work) {
   return static_cast<int>(std::min<long long>(kTableThreads, std::max<long long>(128, (work + 31) / 32 * 32)));
 }
 
-// Workspace of the paged attention: per block of the launch the unit it began
-// and two partial results of a row tile's heads.
-size_t paged_workspace(int group, int D) {
-  const size_t rows = 2 * static_cast<size_t>(std::min(group, 32)) * kPagedMaxBlocks;
-  return kPagedMaxBlocks * sizeof(int4) + rows * (sizeof(float2) + D * sizeof(float));
-}
-
 // Strides of a cache (16-bit elements, multiples of 8) in units of 16 bytes;
 // false if one does not fit 32 bits. A single page's or head's is not used.
 bool to_units(const Strides& s, int P, int Hkv, Units* u) {
@@ -297,44 +290,68 @@ int paged_cluster(long long units, long long most, int sms) {
   return 0;
 }
 
+// How a call is cut: query heads of a row tile, units, steps of a full row, blocks
+// of a cluster (0: the line) and blocks of the launch.
+struct PagedPlan {
+  int rows, row_tiles, cluster;
+  long long units, most, blocks;
+};
+
+PagedPlan paged_plan(int B, int Hq, int Hkv, int W, int D, int page, int sms) {
+  const int group = Hq / Hkv, step = D == 64 ? PagedCfg<64>::STEP : PagedCfg<128>::STEP;
+  PagedPlan p{};
+  p.rows = group <= 8 ? 8 : group <= 16 ? 16 : 32;
+  p.row_tiles = (group + p.rows - 1) / p.rows;
+  p.units = static_cast<long long>(B) * Hkv * p.row_tiles;
+  p.most = (W * page + step - 1) / step;
+  p.cluster = paged_cluster(p.units, p.most, sms);
+  // the line: two blocks an SM, fewer where the table has no room for so many steps
+  p.blocks = p.cluster ? p.units * p.cluster
+                       : static_cast<long long>(std::min<double>(
+                             std::min(2 * sms, kPagedMaxBlocks), static_cast<double>(p.units) * p.most));
+  return p;
+}
+
+// Bytes of the line's workspace: kPagedMaxBlocks records and, per block, two
+// partial results of a row tile's heads. Clusters need none.
+size_t paged_workspace(const PagedPlan& p, int group, int D) {
+  if (p.cluster) return 0;
+  const size_t rows = 2 * static_cast<size_t>(std::min(group, p.rows)) * kPagedMaxBlocks;
+  return kPagedMaxBlocks * sizeof(int4) + rows * (sizeof(float2) + D * sizeof(float));
+}
+
 template <int D, bool BF, int ROWS>
-int paged_attn_launch(PagedAttnArgs& a, int sms, void* stream) {
+int paged_attn_launch(const PagedAttnArgs& a, const PagedPlan& p, void* stream) {
   using C = PagedCfg<D>;
-  const int group = a.Hq / a.Hkv;
-  a.row_tiles = (group + ROWS - 1) / ROWS;
-  const long long units = static_cast<long long>(a.B) * a.Hkv * a.row_tiles;
-  const long long most = (a.W * a.page + C::STEP - 1) / C::STEP;
-  if (const int c = paged_cluster(units, most, sms))
-    return launch_after(paged_attn_kernel<D, BF, ROWS, true>, "paged_attn_kernel", units * c, 128, C::SMEM,
-                        c, stream, a);
-  // two blocks an SM, fewer where the table has no room for so many steps
-  const int blocks = static_cast<int>(std::min<double>(std::min(2 * sms, kPagedMaxBlocks),
-                                                       static_cast<double>(units) * most));
+  const auto blocks = static_cast<unsigned>(p.blocks);
+  if (p.cluster)
+    return launch_after(paged_attn_kernel<D, BF, ROWS, true>, "paged_attn_kernel", blocks, 128, C::SMEM,
+                        p.cluster, stream, a);
   if (int st = launch_after(paged_attn_kernel<D, BF, ROWS, false>, "paged_attn_kernel", blocks, 128, C::SMEM,
                             0, stream, a))
     return st;
-  if (most == 1) return FA_B200_OK;   // nothing is cut
+  if (p.most == 1) return FA_B200_OK;   // nothing is cut
   // few units: many parts each, so 16 columns a block and 16 threads for each of them
-  const int most_cols = 8 * units <= blocks ? 16 : kJoinThreads;
-  const int cols = std::min(group, ROWS) * (D / 4);
+  const int most_cols = 8 * p.units <= p.blocks ? 16 : kJoinThreads;
+  const int cols = std::min(a.Hq / a.Hkv, ROWS) * (D / 4);
   return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel",
-                      dim3(static_cast<unsigned>(std::min<long long>(units, blocks)),
+                      dim3(static_cast<unsigned>(std::min(p.units, p.blocks)),
                            (cols + most_cols - 1) / most_cols),
                       kJoinThreads, 0, 0, stream, a, ROWS, most_cols);
 }
 
 template <int D, bool BF>
-int paged_attn_impl(PagedAttnArgs& a, void* workspace, void* stream) {
-  int dev = 0, sms = 0;
-  if (int st = device_setup(&dev, &a.err, &sms)) return st;
-  const int group = a.Hq / a.Hkv;
-  const size_t rows = 2 * static_cast<size_t>(std::min(group, 32)) * kPagedMaxBlocks;
-  a.split = static_cast<int4*>(workspace);
-  a.part_o = reinterpret_cast<float*>(a.split + kPagedMaxBlocks);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
-  if (group <= 8) return paged_attn_launch<D, BF, 8>(a, sms, stream);
-  if (group <= 16) return paged_attn_launch<D, BF, 16>(a, sms, stream);
-  return paged_attn_launch<D, BF, 32>(a, sms, stream);
+int paged_attn_impl(PagedAttnArgs& a, const PagedPlan& p, void* workspace, void* stream) {
+  a.row_tiles = p.row_tiles;
+  if (!p.cluster) {
+    const size_t rows = 2 * static_cast<size_t>(std::min(a.Hq / a.Hkv, p.rows)) * kPagedMaxBlocks;
+    a.split = static_cast<int4*>(workspace);
+    a.part_o = reinterpret_cast<float*>(a.split + kPagedMaxBlocks);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
+  }
+  if (p.rows == 8) return paged_attn_launch<D, BF, 8>(a, p, stream);
+  if (p.rows == 16) return paged_attn_launch<D, BF, 16>(a, p, stream);
+  return paged_attn_launch<D, BF, 32>(a, p, stream);
 }
 
 // An fp32 dQ is produced by the fused kernel: one pass, dQ added into the
@@ -1064,7 +1081,10 @@ int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b2
 
 size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size) {
   if (fab::check_shape(B, Hq, Hkv, 1, D) || fab::check_pages(1, W, page_size)) return 0;
-  return fab::paged_workspace(Hq / Hkv, D);
+  int dev = 0, sms = 0;
+  int* err = nullptr;
+  if (fab::device_setup(&dev, &err, &sms) != FA_B200_OK) return 0;
+  return fab::paged_workspace(fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms), Hq / Hkv, D);
 }
 
 int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, fa_b200_strides skc,
@@ -1080,7 +1100,6 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
   if (int st = fab::check_pages(P, W, page_size)) return st;
   if (dtype != FA_B200_DTYPE_FP16 && dtype != FA_B200_DTYPE_BF16) return FA_B200_ERR_DTYPE;
   if (static_cast<long long>(B) * Hq > 0x7fffffffll) return FA_B200_ERR_TOO_LARGE;
-  if (!workspace || workspace_bytes < fab::paged_workspace(Hq / Hkv, D)) return FA_B200_ERR_WORKSPACE;
   fab::PagedAttnArgs a{};
   a.q = static_cast<const uint16_t*>(q);
   a.k_cache = static_cast<const uint4*>(k_cache);
@@ -1097,12 +1116,17 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
       !fab::strides_ok(a.so, 2) || !fab::strides_ok(sk, 2) || !fab::strides_ok(sv, 2))
     return FA_B200_ERR_ALIGNMENT;
   if (!fab::to_units(sk, P, Hkv, &a.skc) || !fab::to_units(sv, P, Hkv, &a.svc)) return FA_B200_ERR_TOO_LARGE;
+  int dev = 0, sms = 0;
+  if (int st = fab::device_setup(&dev, &a.err, &sms)) return st;
+  const fab::PagedPlan plan = fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms);
+  const size_t need = fab::paged_workspace(plan, Hq / Hkv, D);
+  if (need && (!workspace || workspace_bytes < need)) return FA_B200_ERR_WORKSPACE;
   const bool bf = dtype == FA_B200_DTYPE_BF16;
   if (D == 64)
-    return bf ? fab::paged_attn_impl<64, true>(a, workspace, stream)
-              : fab::paged_attn_impl<64, false>(a, workspace, stream);
-  return bf ? fab::paged_attn_impl<128, true>(a, workspace, stream)
-            : fab::paged_attn_impl<128, false>(a, workspace, stream);
+    return bf ? fab::paged_attn_impl<64, true>(a, plan, workspace, stream)
+              : fab::paged_attn_impl<64, false>(a, plan, workspace, stream);
+  return bf ? fab::paged_attn_impl<128, true>(a, plan, workspace, stream)
+            : fab::paged_attn_impl<128, false>(a, plan, workspace, stream);
 }
 
 size_t fa_b200_backward_workspace_bytes(int B, int Hq, int N) {

@@ -74,10 +74,10 @@ def _caches(k_cache, v_cache):
     for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         if not isinstance(t, torch.Tensor) or t.dim() != 4:
             raise RuntimeError(f"{name} must be (P, Hkv, page_size, D)")
-        if t.dtype not in _KINDS:
-            raise RuntimeError(f"{name} must be fp16 or bf16")
-    shape = k_cache.shape
-    if shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
+    dtype, shape = k_cache.dtype, k_cache.shape
+    if dtype not in _KINDS:
+        raise RuntimeError("k_cache must be fp16 or bf16")
+    if shape != v_cache.shape or v_cache.dtype is not dtype:
         raise RuntimeError("k_cache and v_cache must have one shape and one dtype")
     P, Hkv, page_size, D = shape
     if D != 64 and D != 128:
@@ -96,29 +96,28 @@ def _strides(t, batch, head, row, d):
     """fa_b200_strides of a 16-bit tensor with these strides, None where 16-byte
     accesses cannot address it. The common case of _lib.strides_of without its
     look at every size; that one decides where a stride of this does not fit."""
-    if d == 1 and (batch | head | row) & 7 == 0 and min(batch, head, row) > 0 and not t.data_ptr() & 15:
+    if d == 1 and not (batch | head | row) & 7 and batch and head and row and not t.data_ptr() & 15:
         return _lib.Strides(batch, head, row)
     return _lib.strides_of(t) if t.dim() == 4 else None
 
 
-def _on_device(**tensors):
+def _on_device(names, *tensors):
     """Index of the one GPU that holds all tensors."""
-    first = None
-    for name, t in tensors.items():
-        dev = t.get_device()
-        if dev < 0:
+    dev = tensors[0].get_device()
+    for t, name in zip(tensors, names):
+        if t.get_device() < 0:
             raise RuntimeError(f"{name} must be a CUDA tensor")
-        if first is None:
-            first = dev
-        elif dev != first:
-            raise RuntimeError(f"{name} must be on cuda:{first}, got {t.device}")
-    return first
+        if t.get_device() != dev:
+            raise RuntimeError(f"{name} must be on cuda:{dev}, got {t.device}")
+    return dev
 
 
 def _no_grad(*tensors):
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError("the paged cache has no backward: call it under torch.no_grad() or "
-                           "detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError("the paged cache has no backward: call it under torch.no_grad() or "
+                                   "detach its inputs")
 
 
 def _call(dev, name, *args):
@@ -187,8 +186,8 @@ def paged_extend(new_lens, lens, block_table, free_pages, free_count, page_size,
     total = int(total_tokens)
     if not 0 <= total <= 0x7fffffff:
         raise RuntimeError(f"total_tokens must be in [0, 2**31), got {total}")
-    dev = _on_device(lens=lens, new_lens=new_lens, block_table=block_table, free_pages=free_pages,
-                     free_count=free_count)
+    dev = _on_device(("lens", "new_lens", "block_table", "free_pages", "free_count"),
+                     lens, new_lens, block_table, free_pages, free_count)
     ws, (slots, granted), lens_out, free_count_out = _outputs(lens, lens_out, free_count_out, total, B)
     _call(dev, "fa_b200_paged_extend", new_lens.data_ptr(), lens.data_ptr(), block_table.data_ptr(),
           stride, free_pages.data_ptr(), free_count.data_ptr(), slots.data_ptr(), granted.data_ptr(),
@@ -206,8 +205,8 @@ def paged_release(finished, lens, block_table, free_pages, free_count, page_size
     tensors or the caller's, as in paged_extend."""
     B, W, stride, P = _requests(lens, block_table, free_pages, free_count, page_size)
     _ints(finished, "finished", (B,), torch.bool)
-    dev = _on_device(lens=lens, finished=finished, block_table=block_table, free_pages=free_pages,
-                     free_count=free_count)
+    dev = _on_device(("lens", "finished", "block_table", "free_pages", "free_count"),
+                     lens, finished, block_table, free_pages, free_count)
     ws, _, lens_out, free_count_out = _outputs(lens, lens_out, free_count_out)
     _call(dev, "fa_b200_paged_release", finished.data_ptr(), lens.data_ptr(), block_table.data_ptr(),
           stride, free_pages.data_ptr(), free_count.data_ptr(), lens_out.data_ptr(),
@@ -236,7 +235,7 @@ def paged_append(k, v, slots, k_cache, v_cache):
     if k_cache.data_ptr() == v_cache.data_ptr():
         raise RuntimeError("k_cache and v_cache must be different memory")
     _no_grad(k, v, k_cache, v_cache)
-    dev = _on_device(k_cache=k_cache, v_cache=v_cache, k=k, v=v, slots=slots)
+    dev = _on_device(("k_cache", "v_cache", "k", "v", "slots"), k_cache, v_cache, k, v, slots)
     if T == 0:
         return
     (k, sk), (v, sv) = _token_rows(k), _token_rows(v)
@@ -260,8 +259,9 @@ def _token_rows(t):
 
 
 @functools.lru_cache(maxsize=1024)
-def _attn_workspace_bytes(B, Hq, Hkv, W, D, page_size):
-    return _lib.lib().fa_b200_paged_attn_workspace_bytes(B, Hq, Hkv, W, D, page_size)
+def _attn_workspace_bytes(dev, B, Hq, Hkv, W, D, page_size):
+    with torch.cuda.device(dev):
+        return _lib.lib().fa_b200_paged_attn_workspace_bytes(B, Hq, Hkv, W, D, page_size)
 
 
 def paged_attn(q, k_cache, v_cache, block_table, lens):
@@ -283,7 +283,8 @@ def paged_attn(q, k_cache, v_cache, block_table, lens):
     W, stride = _table(block_table, B)
     _check_page_size(page_size, P, W)
     _no_grad(q, k_cache, v_cache)
-    dev = _on_device(q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, lens=lens)
+    dev = _on_device(("q", "k_cache", "v_cache", "block_table", "lens"),
+                     q, k_cache, v_cache, block_table, lens)
     batch, head, d = q.stride()
     sq = _strides(q, batch, head, 8, d)          # no row axis
     if sq is None:
@@ -293,11 +294,12 @@ def paged_attn(q, k_cache, v_cache, block_table, lens):
             sq = _lib.strides_of(q.unsqueeze(2))
     o = q.new_empty(shape)
     lse = q.new_empty((B, Hq), dtype=torch.float32)
-    ws_bytes = _attn_workspace_bytes(B, Hq, Hkv, W, D, page_size)
-    ws = lens.new_empty(ws_bytes // 4)
+    ws_bytes = _attn_workspace_bytes(dev, B, Hq, Hkv, W, D, page_size)
+    ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None
     _call(dev, "fa_b200_paged_attn", q.data_ptr(), sq, k_cache.data_ptr(), skc, v_cache.data_ptr(), svc,
           block_table.data_ptr(), stride, lens.data_ptr(), o.data_ptr(), _lib.Strides(Hq * D, D, D),
-          lse.data_ptr(), ws.data_ptr(), ws_bytes, B, Hq, Hkv, D, P, W, page_size, _KINDS[q.dtype])
+          lse.data_ptr(), ws.data_ptr() if ws_bytes else None, ws_bytes, B, Hq, Hkv, D, P, W, page_size,
+          _KINDS[q.dtype])
     return o, lse
 
 

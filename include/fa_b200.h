@@ -193,7 +193,9 @@ int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b2
                          fa_b200_strides svc, int T, int Hkv, int D, int P, int page_size,
                          int dtype, void* stream);
 
-/* Bytes of device workspace for fa_b200_paged_attn (0: none needed). */
+/* Bytes of device workspace for fa_b200_paged_attn with these sizes on the current
+ * device (0: none needed, or the sizes or the device are refused there). The
+ * workspace serves one call at a time; nothing in it has to start at zero. */
 size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size);
 
 /* Attention of one token per request over its cached tokens 0 .. lens[r] - 1

@@ -39,6 +39,8 @@ import _lib
 _I32 = torch.int32
 _KINDS = {torch.float16: _lib.DTYPE_FP16, torch.bfloat16: _lib.DTYPE_BF16}
 _DENSE = torch.contiguous_format
+# a structure of three numbers costs ctypes as much as a small allocation
+_Strides = functools.lru_cache(maxsize=4096)(_lib.Strides)
 
 
 def _ints(t, name, shape, dtype=_I32):
@@ -97,7 +99,7 @@ def _strides(t, batch, head, row, d):
     accesses cannot address it. The common case of _lib.strides_of without its
     look at every size; that one decides where a stride of this does not fit."""
     if d == 1 and not (batch | head | row) & 7 and batch and head and row and not t.data_ptr() & 15:
-        return _lib.Strides(batch, head, row)
+        return _Strides(batch, head, row)
     return _lib.strides_of(t) if t.dim() == 4 else None
 
 
@@ -297,7 +299,7 @@ def paged_attn(q, k_cache, v_cache, block_table, lens):
     ws_bytes = _attn_workspace_bytes(dev, B, Hq, Hkv, W, D, page_size)
     ws = lens.new_empty(ws_bytes // 4) if ws_bytes else None
     _call(dev, "fa_b200_paged_attn", q.data_ptr(), sq, k_cache.data_ptr(), skc, v_cache.data_ptr(), svc,
-          block_table.data_ptr(), stride, lens.data_ptr(), o.data_ptr(), _lib.Strides(Hq * D, D, D),
+          block_table.data_ptr(), stride, lens.data_ptr(), o.data_ptr(), _Strides(Hq * D, D, D),
           lse.data_ptr(), ws.data_ptr() if ws_bytes else None, ws_bytes, B, Hq, Hkv, D, P, W, page_size,
           _KINDS[q.dtype])
     return o, lse

@@ -109,6 +109,8 @@ void set_smem_all() {
   set_smem_paged<128, BF, 8>();
   set_smem_paged<128, BF, 16>();
   set_smem_paged<128, BF, 32>();
+  set_smem(paged_join_kernel<64, BF>, 0);
+  set_smem(paged_join_kernel<128, BF>, 0);
 }
 
 // One-time, per-device set-up with that device current: architecture check,
@@ -145,6 +147,10 @@ int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr) {
         st.err = static_cast<int*>(addr);
         set_smem_all<false>();
         set_smem_all<true>();
+        // loads the paged kernels that need no opt-in: a first call may be captured
+        set_smem(extend_kernel, 0), set_smem(extend_fill_kernel, 0);
+        set_smem(release_kernel, 0), set_smem(release_fill_kernel, 0);
+        set_smem(append_kernel<64>, 0), set_smem(append_kernel<128>, 0);
         st.status = (cudaGetLastError() == cudaSuccess) ? FA_B200_OK : FA_B200_ERR_DEVICE;
       }
     }

@@ -586,3 +586,34 @@ def test_decode_step_in_a_graph(cuda):
             assert torch.equal(eager.block_table, graphed.block_table)
             assert torch.equal(eager.k, graphed.k) and torch.equal(eager.v, graphed.v)
     assert state[0][0].lens.tolist() == [47, 70, 41, 56, 0]
+
+
+def test_first_calls_may_be_captured(cuda):
+    """In a process of its own, the operators' very first calls inside a captured graph."""
+    code = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+import fa_p100_paged as paged
+dev = torch.device("cuda", 0)
+c = paged.PagedKVCache(1, 1, 64, 4000, 3, 20000, 16, torch.float16, dev)
+new = torch.tensor([9000, 40, 1], dtype=torch.int32, device=dev)
+fin = torch.tensor([True, False, True], device=dev)
+k, q = torch.ones(9041, 1, 64, device=dev).half(), torch.ones(3, 1, 64, device=dev).half()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    c.extend(new, 9041)
+    c.append(0, k, k)
+    o = c.attn(0, q)
+    c.release(fin)
+g.replay()
+torch.cuda.synchronize()
+assert c.lens.tolist() == [0, 40, 0] and int(c.free_count) == 4000 - 3
+assert torch.equal(o, torch.ones_like(o))
+"""
+    import os
+    import subprocess
+    import sys
+    res = subprocess.run([sys.executable, "-c", code, os.path.dirname(paged.__file__)],
+                         capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr[-2000:]

@@ -85,5 +85,43 @@ def build(force=False, verbose=False, checked=None):
     return path
 
 
+# The paged operators' torch module (csrc/fa_paged_py.cpp), built against the
+# installed torch by the host compiler.
+BINDING_SOURCE = os.path.join(CSRC, "fa_paged_py.cpp")
+BINDING_PATH = os.path.join(HERE, "_fa_paged.so")
+
+
+def binding_up_to_date():
+    if not os.path.exists(BINDING_PATH):
+        return False
+    built = os.path.getmtime(BINDING_PATH)
+    return all(os.path.getmtime(s) <= built
+               for s in (BINDING_SOURCE, os.path.join(INCLUDE, "fa_b200.h")))
+
+
+def build_binding(force=False):
+    """Compile csrc/fa_paged_py.cpp into _fa_paged.so, a CPython module over the
+    installed torch. Returns its path."""
+    if not force and binding_up_to_date():
+        return BINDING_PATH
+    import sysconfig
+
+    import torch
+    home = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    tmp = f"{BINDING_PATH}.{os.getpid()}.tmp"
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f"-I{home}/include", f"-I{home}/include/torch/csrc/api/include",
+           f"-I{sysconfig.get_path('include')}", f"-I{cuda}/include", BINDING_SOURCE, "-o", tmp,
+           f"-L{home}/lib", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed building _fa_paged.so:\n" + res.stdout + res.stderr)
+    os.replace(tmp, BINDING_PATH)
+    return BINDING_PATH
+
+
 if __name__ == "__main__":
     print(build(force=True, verbose=True))
+    print(build_binding(force=True))

@@ -284,13 +284,15 @@ bool to_units(const Strides& s, int P, int Hkv, Units* u) {
 //   20 requests (160 blocks) of 512 tokens 10.7 / 12.7, of 1024 17.4 / 16.5
 //   40 requests (two blocks a unit, in waves) of 256 tokens 14.9 / 12.9
 //   1 kv head, D=64, 1 request: 2048 tokens 5.1 / 6.6, 8192 7.7 / 7.0, 16000 13.2 / 8.4
-// so the steps a block may have to take grow with the part of the GPU in use.
+//   256 units (a block each), D=64, 2048 tokens 25.1 / 28.8, of 1 to 2048 19.2 / 16.8
+// so the steps a block may have to take grow with the part of the GPU in use, where
+// a unit's keys are spread over several blocks.
 int paged_cluster(long long units, long long most, int sms) {
   for (int c = 16; c >= 1; c /= 2) {
     const long long blocks = units * c;
     if (c > 1 && c / 2 >= most) continue;   // no more blocks than steps
     if (blocks > (c == 16 ? sms : 2 * sms)) continue;
-    const int steps = 2 * blocks > 3 * sms ? 16 : 2 * blocks > sms ? 8 : 4;
+    const int steps = c > 1 && 2 * blocks > 3 * sms ? 16 : 2 * blocks > sms ? 8 : 4;
     return most <= static_cast<long long>(c) * steps ? c : 0;
   }
   return 0;
@@ -1014,7 +1016,7 @@ int fa_b200_paged_extend(const int* new_lens, const int* lens, int* block_table,
                           lens_out, free_count_out, table_stride, head,
                           reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size, T};
   const bool wide = T > fab::kExtendWide;
-  const long long runs = (T + fab::kSlotRun - 1ll) / fab::kSlotRun;
+  const long long runs = (static_cast<long long>(T) + fab::kSlotRun - 1) / fab::kSlotRun;
   if (int st = fab::launch_after(fab::extend_kernel, "extend_kernel", 1,
                                  fab::table_threads(wide ? B : std::max<long long>(B, runs)), 0, 0, stream,
                                  a, !wide))

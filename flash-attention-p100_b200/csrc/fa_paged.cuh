@@ -23,10 +23,13 @@ namespace fab {
 // writes that need only their results. The sums are latency: a load, two scans,
 // a store. The writes go by the same block where the host knows that they are
 // few, else by a second launch that fills the GPU and whose start overlaps the
-// first (kExtendWide, kReleaseWide).
+// first (kExtendWide, kReleaseWide). Bound by latency throughout: 64 decoding
+// requests take 2.4 us, 1024 prompts with 1.03 M tokens 11.3 us (4.7 MB read and
+// written), the return of 262 k pages of 2048 requests 7.9 us.
 constexpr int kTableThreads = 1024;
 // Slots (extend), and runs of kReleaseRun table entries (release), above which the
-// second launch pays.
+// second launch pays. Measured, one block against two launches, in us: 4096 slots
+// of 128 requests 4.4 / 5.1, 8192 6.0 / 5.0; 16 runs 4.4 / 5.1, 64 runs 7.5 / 5.2.
 constexpr int kExtendWide = 4096, kReleaseWide = 32;
 // Up to this many tokens a request's own thread writes them (a decoding step);
 // a page holds 16 or more, so they take at most one new page.
@@ -195,7 +198,7 @@ __device__ __forceinline__ void extend_fill(const ExtendArgs& a, const Tok& tok,
     TableRow row = a.rows[r];
     int slot[kSlotRun];
     const int in = t - row.tok;
-    if (in + kSlotRun <= row.count) {   // one request
+    if (row.count - in >= kSlotRun) {   // one request
       const int pos = row.len + in, j = pos / a.page, off = pos - j * a.page;
       const int id0 = page_id(a, row, r, j, free);
       const int id1 = off + kSlotRun > a.page ? page_id(a, row, r, j + 1, free) : -1;
@@ -401,6 +404,14 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // Inside a block each warp takes KEYS of a step's keys into a ring of its own
 // (cp.async, 16 bytes a lane), three steps deep, across unit borders too: the
 // loads never drain, and warps meet only where a unit ends.
+//
+// Measured: 64 ragged requests of 32/8 heads of 128 (1.0 GB of cache) 155 us, 6.45
+// TB/s or 98% of the measured copy, DRAM traffic equal to the cache's bytes, a fifth
+// of the tensor pipe; one request of 131001 tokens 85 us, 6.3 TB/s; one of 1000
+// tokens 6.0 us, a chain of dependent loads (length, page, keys). Groups of 17 to
+// 32 heads, 0.26 GB: 85 us against 52 for 16, bound by the latency of two
+// fragments' products at 8 warps an SM.
+
 // Strides of a cache in units of 16 bytes (page, head, token): products of 32
 // bits, one instruction each, that still span 64 GB.
 struct Units {
@@ -609,8 +620,8 @@ struct PagedAt {
 };
 
 // ROWS query heads of a group per unit: 8 (half of an m16 fragment, whose other
-// half takes the weights' second terms), 16 (one fragment) or 32 (two); a group above 32 is cut into
-// row tiles, each of which reads the cache again.
+// half takes the weights' second terms), 16 (one fragment) or 32 (two); a group
+// above 32 is cut into row tiles, each of which reads the cache again.
 template <int D, bool BF, int ROWS, bool CLUSTER>
 __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) {
   using C = PagedCfg<D>;
@@ -811,6 +822,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     }
     cp_async_commit();
   };
+
   // ---- per unit state ----
   uint32_t qf[MT][D / 16][4];
   float o[MT][D / 8][4], m[MT][E], l[MT][E];

@@ -164,6 +164,19 @@ def test_extend_odd_values(cuda):
                [0, 1, 3, 4, 5, 6, 7, 8], 8, ps, 41)
 
 
+def test_extend_most_tokens(cuda):
+    """A call of 2^31 - 1 tokens: a request too long for its row, and one that fits
+    behind which the slots end."""
+    table = i32([[-1] * 4, [-1] * 4], cuda)
+    stack, count, total = i32([5, 4, 3, 2, 1, 0], cuda), i32([6], cuda), 2 ** 31 - 1
+    slots, granted, lens, left = paged.paged_extend(i32([2 ** 31 - 41, 40], cuda), i32([0, 0], cuda), table, stack,
+                                                    count, 16, total)
+    assert granted.tolist() == [0, 40] and lens.tolist() == [0, 40] and left.tolist() == [3]
+    assert slots[-40:].tolist() == list(range(40)) and int(slots[:-40].max()) == -1
+    slots, granted, _, left = paged.paged_extend(i32([total, 0], cuda), i32([0, 40], cuda), table, stack, left, 16, total)
+    assert granted.tolist() == [0, 0] and left.tolist() == [3] and int(slots.max()) == -1
+
+
 RELEASE = [(1, 1, 16, 16, 1, 0), (7, 9, 16, 140, 2, 1), (64, 40, 48, 1500, 3, 2),
            (1024, 10, 32, 300, 1, 3), (2100, 7, 16, 100, 2, 4), (4, 3000, 16, 48000, 1, 5)]
 

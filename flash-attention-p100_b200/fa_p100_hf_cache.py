@@ -7,7 +7,7 @@
     model.generate(ids, past_key_values=cache, use_cache=True, max_new_tokens=100)
 
 No counterpart in the reference, whose backend refuses every cache
-(fa_p100_hf.py:103-105). A prompt runs through flash_attn as without a cache and
+(fa_p100_hf.py:64-105). A prompt runs through flash_attn as without a cache and
 leaves its keys and values in the pages; every token after it runs through
 fa_p100_paged.paged_attn over them. All sequences of a batch have one length, as
 the backend takes no padding. What it cannot do raises: a second prompt on a

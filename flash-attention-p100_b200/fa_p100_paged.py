@@ -1,6 +1,6 @@
 """Generation with a paged key-value cache: what a model needs after `flash_attn`
 has read its prompt. The reference has no cache (its HuggingFace backend refuses
-one, fa_p100_hf.py:103-105); these operators have no counterpart there.
+one, fa_p100_hf.py:64-105); these operators have no counterpart there.
 
     cache = PagedKVCache(layers, Hkv, D, pages, batch, max_len)
     cache.extend(new_lens, total_tokens)        # pages and slots for the new tokens

@@ -149,7 +149,8 @@ int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr) {
         set_smem_all<true>();
         // loads the paged kernels that need no opt-in: a first call may be captured
         set_smem(extend_kernel, 0), set_smem(extend_fill_kernel, 0);
-        set_smem(release_kernel, 0), set_smem(release_fill_kernel, 0);
+        set_smem(release_kernel<true>, 0), set_smem(release_kernel<false>, 0);
+        set_smem(release_fill_kernel, 0);
         set_smem(append_kernel<64>, 0), set_smem(append_kernel<128>, 0);
         st.status = (cudaGetLastError() == cudaSuccess) ? FA_B200_OK : FA_B200_ERR_DEVICE;
       }
@@ -1047,12 +1048,11 @@ int fa_b200_paged_release(const unsigned char* finished, const int* lens, const 
                            free_count_out, table_stride, head,
                            reinterpret_cast<fab::TableRow*>(head + 1), B, W, P, page_size};
   const long long runs = static_cast<long long>(B) * ((W + fab::kReleaseRun - 1) / fab::kReleaseRun);
-  const bool wide = runs > fab::kReleaseWide;
-  if (int st = fab::launch_after(fab::release_kernel, "release_kernel", 1,
-                                 fab::table_threads(wide ? B : std::max<long long>(B, 32 * runs)), 0, 0,
-                                 stream, a, !wide))
+  if (runs <= fab::kReleaseWide)
+    return fab::launch_after(fab::release_kernel<true>, "release_kernel", 1, fab::kTableThreads, 0, 0, stream, a);
+  if (int st = fab::launch_after(fab::release_kernel<false>, "release_kernel", 1, fab::table_threads(B), 0, 0,
+                                 stream, a))
     return st;
-  if (!wide) return FA_B200_OK;
   return fab::launch_after(fab::release_fill_kernel, "release_fill_kernel",
                            std::min<long long>((runs + 7) / 8, 8 * sms), 256, 0, 0, stream, a);
 }

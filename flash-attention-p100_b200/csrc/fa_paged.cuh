@@ -27,10 +27,12 @@ namespace fab {
 // requests take 2.4 us, 1024 prompts with 1.03 M tokens 11.3 us (4.7 MB read and
 // written), the return of 262 k pages of 2048 requests 7.9 us.
 constexpr int kTableThreads = 1024;
-// Slots (extend), and runs of kReleaseRun table entries (release), above which the
-// second launch pays. Measured, one block against two launches, in us: 4096 slots
-// of 128 requests 4.4 / 5.1, 8192 6.0 / 5.0; 16 runs 4.4 / 5.1, 64 runs 7.5 / 5.2.
-constexpr int kExtendWide = 4096, kReleaseWide = 32;
+// Slots (extend), and runs of kReleaseRun table entries of all requests (release),
+// above which the second launch pays. Measured, one block against two launches, in
+// us: 4096 slots of 128 requests 4.4 / 5.1, 8192 6.0 / 5.0; 64 requests of up to 512
+// pages (128 runs) 3.8 / 4.2 when every eighth ends, 9.2 / 5.4 when all do, and 2 us of
+// host time less; 256 requests of up to 256 pages (256 runs) 5.2 / 5.2 and 19.2 / 5.4.
+constexpr int kExtendWide = 4096, kReleaseWide = 128;
 // Up to this many tokens a request's own thread writes them (a decoding step);
 // a page holds 16 or more, so they take at most one new page.
 constexpr int kSlotsByRow = 4;
@@ -277,66 +279,83 @@ struct ReleaseArgs {
   int B, W, P, page;
 };
 
-// Which requests give pages back and where those start.
-__device__ __forceinline__ void release_rows(const ReleaseArgs& a) {
+// Entries of a row that a warp copies at a time.
+constexpr int kReleaseRun = 256;
+
+// Entries [j0, j0 + kReleaseRun) of row r onto the stack, by one warp. `row` has
+// the row's count and first page, `pages` is where the call's pages end.
+__device__ __forceinline__ void release_run(const ReleaseArgs& a, const TableRow& row, int r, int j0, int free,
+                                            int pages) {
+  // a clipped first page is behind the stack's end
+  const long long end = min(min(static_cast<long long>(row.count), static_cast<long long>(j0) + kReleaseRun),
+                            static_cast<long long>(pages) - row.page);
+  const int* from = a.table + r * a.table_stride;
+  int* to = a.free_pages + free + row.page;
+#pragma unroll 8
+  for (long long j = j0 + static_cast<int>(threadIdx.x & 31); j < end; j += 32) to[j] = from[j];
+}
+
+// Which requests give pages back and where those start. With FILL the block also
+// copies them, the finished requests of kTableThreads rows at a time from a list
+// in shared memory; else `rows` and `head` tell release_fill_kernel.
+template <bool FILL>
+__global__ void __launch_bounds__(kTableThreads) release_kernel(const ReleaseArgs a) {
   __shared__ long long sums[32];
-  const int free = clamp_count(*a.free_count, a.P);
+  __shared__ TableRow s_row[FILL ? kTableThreads : 1];
+  __shared__ int s_index[FILL ? kTableThreads : 1];
+  wait_for_prior_launch();
+  const int free = clamp_count(*a.free_count, a.P), room = a.P - free;
+  // more pages than the stack has room for cannot come from one pool: the rest
+  // are dropped
   long long page0 = 0;
   for (int r0 = 0; r0 < a.B; r0 += static_cast<int>(blockDim.x)) {
     const int r = r0 + static_cast<int>(threadIdx.x);
     const bool done = r < a.B && a.finished[r] != 0;
     const int len = r < a.B ? a.lens[r] : 0;
     const int n = done ? (min(max(len, 0), a.W * a.page) + a.page - 1) / a.page : 0;
+    // two sums in one: pages below bit 48, requests that have any above it
+    constexpr int kCount = 48;
     long long all;
-    const long long c = page0 + block_sum(n, sums, &all);
-    page0 += all;
+    const long long sum = block_sum(n + (static_cast<long long>(n > 0) << kCount), sums, &all);
+    const long long c = page0 + (sum & ((1ll << kCount) - 1));
+    const TableRow row{0, clip_int(c - n), len, n};
     if (r < a.B) {
-      a.rows[r] = TableRow{0, clip_int(c - n), len, n};
+      if (!FILL) a.rows[r] = row;
       a.lens_out[r] = done ? 0 : len;
     }
+    if (FILL) {
+      if (n > 0) {
+        s_row[(sum >> kCount) - 1] = row;
+        s_index[(sum >> kCount) - 1] = r;
+      }
+      __syncthreads();
+      const int listed = static_cast<int>(all >> kCount), runs = (a.W + kReleaseRun - 1) / kReleaseRun;
+      const long long items = static_cast<long long>(listed) * runs;
+      for (long long i = threadIdx.x >> 5; i < items; i += blockDim.x >> 5) {
+        const int at = static_cast<int>(i / runs);
+        release_run(a, s_row[at], s_index[at], static_cast<int>(i - static_cast<long long>(at) * runs) * kReleaseRun,
+                    free, room);
+      }
+    }
+    page0 += all & ((1ll << kCount) - 1);
   }
   if (threadIdx.x == 0) {
-    // more pages than the stack has room for cannot come from one pool: the
-    // rest are dropped
-    const int back = static_cast<int>(min(page0, static_cast<long long>(a.P - free)));
-    *a.head = TableHead{back, free, 0, 0};
+    const int back = static_cast<int>(min(page0, static_cast<long long>(room)));
+    if (!FILL) *a.head = TableHead{back, free, 0, 0};
     *a.free_out = free + back;
   }
 }
 
-// The pages onto the stack: warp `first`, `first + step`, ... of the launch each
-// copy up to kReleaseRun entries of a row.
-constexpr int kReleaseRun = 256;
-
-__device__ __forceinline__ void release_fill(const ReleaseArgs& a, long long first, long long step) {
-  const int free = a.head->free, pages = a.head->pages, lane = threadIdx.x & 31;
-  const int runs = (a.W + kReleaseRun - 1) / kReleaseRun;
-  const long long all = static_cast<long long>(a.B) * runs;
-  for (long long i = first; i < all; i += step) {
-    const int r = static_cast<int>(i / runs), j0 = static_cast<int>(i - static_cast<long long>(r) * runs) * kReleaseRun;
-    const TableRow row = a.rows[r];
-    if (j0 >= row.count) continue;
-    // a clipped first page is behind the stack's end
-    const long long end = min(min(static_cast<long long>(row.count), static_cast<long long>(j0) + kReleaseRun),
-                              static_cast<long long>(pages) - row.page);
-    const int* from = a.table + r * a.table_stride;
-    int* to = a.free_pages + free + row.page;
-#pragma unroll 8
-    for (long long j = j0 + lane; j < end; j += 32) to[j] = from[j];
-  }
-}
-
-__global__ void __launch_bounds__(kTableThreads) release_kernel(const ReleaseArgs a, int fill) {
-  wait_for_prior_launch();
-  release_rows(a);
-  if (!fill) return;
-  __syncthreads();
-  release_fill(a, threadIdx.x >> 5, blockDim.x >> 5);
-}
-
 __global__ void __launch_bounds__(256) release_fill_kernel(const ReleaseArgs a) {
   wait_for_prior_launch();
-  release_fill(a, blockIdx.x * 8ll + (threadIdx.x >> 5), gridDim.x * 8ll);
+  const int free = a.head->free, pages = a.head->pages;
+  const int runs = (a.W + kReleaseRun - 1) / kReleaseRun;
+  const long long items = static_cast<long long>(a.B) * runs;
+  for (long long i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < items; i += gridDim.x * 8ll) {
+    const int r = static_cast<int>(i / runs), j0 = static_cast<int>(i - static_cast<long long>(r) * runs) * kReleaseRun;
+    const TableRow row = a.rows[r];
+    if (j0 < row.count) release_run(a, row, r, j0, free, pages);
+  }
 }
 
 // ---------------------------------------------------------------------------

@@ -178,7 +178,8 @@ def test_extend_most_tokens(cuda):
 
 
 RELEASE = [(1, 1, 16, 16, 1, 0), (7, 9, 16, 140, 2, 1), (64, 40, 48, 1500, 3, 2),
-           (1024, 10, 32, 300, 1, 3), (2100, 7, 16, 100, 2, 4), (4, 3000, 16, 48000, 1, 5)]
+           (1024, 10, 32, 300, 1, 3), (2100, 7, 16, 100, 2, 4), (4, 3000, 16, 48000, 1, 5),
+           (128, 255, 16, 4080, 1, 6), (129, 256, 16, 4096, 1, 7), (100, 20, 16, 320, 5, 8)]
 
 
 @pytest.mark.parametrize("case", RELEASE, ids=lambda c: "-".join(map(str, c)))

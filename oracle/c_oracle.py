@@ -21,7 +21,8 @@ _I = ctypes.c_int
 
 def reference_tree():
     """The reference's source tree: $FA_REFERENCE_TREE, else BASELINE.json's
-    `reference_path`; None when neither names an existing directory."""
+    `reference_path`; None when neither names a directory that holds the sources
+    the oracles are compiled from."""
     path = os.environ.get("FA_REFERENCE_TREE")
     if not path:
         try:
@@ -29,7 +30,8 @@ def reference_tree():
                 path = json.load(f).get("reference_path")
         except (OSError, ValueError):
             path = None
-    return path if path and os.path.isdir(path) else None
+    sources = ("attention.cu", "bwd.cu")
+    return path if path and all(os.path.exists(os.path.join(path, f)) for f in sources) else None
 
 
 def _make(target=None, ref=None):

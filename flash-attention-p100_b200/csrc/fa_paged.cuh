@@ -638,6 +638,119 @@ struct PagedAt {
   int len;
 };
 
+__device__ __forceinline__ int request_len(const PagedAttnArgs& a, int b) {
+  return min(max(a.lens[b], 0), a.W * a.page);
+}
+
+// The result of `heads` heads of a request without a token, by the whole block.
+template <int D, int THREADS>
+__device__ __forceinline__ void empty_row(const PagedAttnArgs& a, int b, int head0, int heads) {
+  for (int i = threadIdx.x; i < heads * (D / 2); i += THREADS)
+    *reinterpret_cast<uint32_t*>(a.o + a.so.at(b, head0 + i / (D / 2), 0) + i % (D / 2) * 2) = 0;
+  for (int h = threadIdx.x; h < heads; h += THREADS)
+    a.lse[static_cast<long long>(b) * a.Hq + head0 + h] = -INFINITY;
+}
+
+// A block's stretch of the line, found by every block for itself.
+struct Line {
+  long long total, end;  // steps of the line; where the stretch ends
+  int blocks;            // blocks that have a stretch
+};
+struct LineShared {
+  long long sums[8], first;  // first: the stretch's first step in its request
+  int b;                     // that request
+};
+
+// Adds up the lengths, divides the line, finds this block's stretch and deals
+// with the requests without a token. Returns the stretch's steps.
+template <int STEP, int D, int THREADS>
+__device__ __forceinline__ long long line_begin(const PagedAttnArgs& a, int units, bool by_unit, Line& line,
+                                                LineShared& shared) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const auto steps = [&](int b) { return (request_len(a, b) + STEP - 1) / STEP; };
+  const int per = (a.B + THREADS - 1) / THREADS;
+  const int b0 = min(static_cast<int>(threadIdx.x) * per, a.B), b1 = min(b0 + per, a.B);
+  long long mine = 0, total = 0;
+  for (int b = b0; b < b1; ++b) mine += static_cast<long long>(steps(b)) * units;
+  long long sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += y;
+  }
+  if (lane == 31) shared.sums[warp] = sum;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) sum += shared.sums[w];
+    total += shared.sums[w];
+  }
+  const int blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total)), c = blockIdx.x;
+  const long long g0 = c < blocks ? c * total / blocks : total;
+  const long long g1 = c < blocks ? (c + 1) * total / blocks : total;
+  long long first = sum - mine;
+  if (first <= g0 && g0 < sum) {
+    int b = b0;
+    for (;; ++b) {
+      const long long n = static_cast<long long>(steps(b)) * units;
+      if (g0 < first + n) break;
+      first += n;
+    }
+    shared.b = b;
+    shared.first = g0 - first;
+  }
+  line.total = total;
+  line.end = g1;
+  line.blocks = blocks;
+  if (!by_unit && threadIdx.x == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (request_len(a, b) != 0) continue;
+    empty_row<D, THREADS>(a, b, 0, a.Hq);
+    if (by_unit)
+      for (int u = threadIdx.x; u < units; u += THREADS) a.split[b * units + u] = make_int4(-1, 0, 0, 0);
+  }
+  __syncthreads();
+  return g1 - g0;
+}
+
+// Where the stretch begins.
+template <int STEP>
+__device__ __forceinline__ PagedAt line_at(const PagedAttnArgs& a, const LineShared& shared) {
+  PagedAt at;
+  at.b = shared.b;
+  at.len = request_len(a, at.b);
+  at.nt = (at.len + STEP - 1) / STEP;
+  const int unit = static_cast<int>(shared.first / at.nt);
+  at.t = static_cast<int>(shared.first - static_cast<long long>(unit) * at.nt);
+  at.head = unit / a.row_tiles;
+  at.rt = unit - at.head * a.row_tiles;
+  return at;
+}
+
+// The unit behind x's on the line.
+template <int STEP>
+__device__ __forceinline__ void next_unit(const PagedAttnArgs& a, PagedAt& x) {
+  x.t = 0;
+  if (++x.rt < a.row_tiles) return;
+  x.rt = 0;
+  if (++x.head < a.Hkv) return;
+  x.head = 0;
+  do x.len = request_len(a, ++x.b); while (x.len == 0);
+  x.nt = (x.len + STEP - 1) / STEP;
+}
+
+// For paged_join_kernel: the unit that begins in this block, `done` its last step
+// here, and the block that holds the unit's last step where it is cut.
+__device__ __forceinline__ void line_record(const PagedAttnArgs& a, const Line& line, const PagedAt& done, bool whole,
+                                            bool by_unit) {
+  if (whole && !by_unit) return;
+  const int unit = (done.b * a.Hkv + done.head) * a.row_tiles + done.rt;
+  const long long last = line.end - 1 + (done.nt - 1 - done.t);
+  a.split[by_unit ? unit : static_cast<int>(blockIdx.x)] =
+      make_int4(whole ? -1 : unit, blockIdx.x,
+                whole ? 0 : static_cast<int>(((last + 1) * line.blocks - 1) / line.total), 0);
+}
+
 // ROWS query heads of a group per unit: 8 (half of an m16 fragment, whose other
 // half takes the weights' second terms), 16 (one fragment) or 32 (two); a group
 // above 32 is cut into row tiles, each of which reads the cache again.
@@ -647,28 +760,19 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   constexpr int MT = ROWS > 16 ? 2 : 1, E = ROWS == 8 ? 1 : 2;  // fragments, rows a thread holds of each
   constexpr float kBias = weight_bias<BF>();
   extern __shared__ __align__(1024) unsigned char smem[];
-  __shared__ long long s_sum[C::WARPS], s_at;
-  __shared__ int s_b, s_valid[C::WARPS][C::STAGES];
+  __shared__ LineShared s_line;
+  __shared__ int s_valid[C::WARPS][C::STAGES];
   __shared__ float2 s_ml[C::WARPS][8];
   __shared__ float2 s_unit_ml[ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
-  const int cap = a.W * a.page;
   const bool by_unit = static_cast<long long>(a.B) * units <= gridDim.x;
   wait_for_prior_launch();
-  const auto length = [&](int b) { return min(max(a.lens[b], 0), cap); };
-  const auto steps = [&](int len) { return (len + C::STEP - 1) / C::STEP; };
-  const auto empty_row = [&](int b, int head0, int heads) {
-    for (int i = threadIdx.x; i < heads * (D / 2); i += 128)
-      *reinterpret_cast<uint32_t*>(a.o + a.so.at(b, head0 + i / (D / 2), 0) + i % (D / 2) * 2) = 0;
-    for (int h = threadIdx.x; h < heads; h += 128)
-      a.lse[static_cast<long long>(b) * a.Hq + head0 + h] = -INFINITY;
-  };
-
   // ---- this block's steps ----
   PagedAt at;
-  long long n_steps, total = 0, g1 = 0;
-  int blocks = 0, rank = 0, ranks = 1;   // ranks: also how many steps on the block's next one is
+  Line line{};
+  long long n_steps;
+  int rank = 0, ranks = 1;   // ranks: also how many steps on the block's next one is
   if constexpr (CLUSTER) {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
     asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(ranks));
@@ -676,71 +780,15 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     at.b = unit / units;
     at.head = (unit - at.b * units) / a.row_tiles;
     at.rt = unit % a.row_tiles;
-    at.len = length(at.b);
-    at.nt = steps(at.len);
+    at.len = request_len(a, at.b);
+    at.nt = (at.len + C::STEP - 1) / C::STEP;
     at.t = rank;     // steps in turn: where a block begins does not depend on the length
     n_steps = at.nt > rank ? (at.nt - rank + ranks - 1) / ranks : 0;
   } else {
-    // every block adds up the lengths itself; [g0, g1) is its stretch of the line
-    const int per = (a.B + 127) / 128;
-    const int b0 = min(static_cast<int>(threadIdx.x) * per, a.B), b1 = min(b0 + per, a.B);
-    long long mine = 0;
-    for (int b = b0; b < b1; ++b) mine += static_cast<long long>(steps(length(b))) * units;
-    long long sum = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += y;
-    }
-    if (lane == 31) s_sum[warp] = sum;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < C::WARPS; ++w) {
-      if (w < warp) sum += s_sum[w];
-      total += s_sum[w];
-    }
-    blocks = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
-    const int c = blockIdx.x;
-    const long long g0 = c < blocks ? c * total / blocks : total;
-    g1 = c < blocks ? (c + 1) * total / blocks : total;
-    n_steps = g1 - g0;
-    long long first = sum - mine;
-    if (first <= g0 && g0 < sum) {
-      int b = b0;
-      for (;; ++b) {
-        const long long n = static_cast<long long>(steps(length(b))) * units;
-        if (g0 < first + n) break;
-        first += n;
-      }
-      s_b = b;
-      s_at = g0 - first;
-    }
-    if (!by_unit && threadIdx.x == 0) a.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-      if (length(b) != 0) continue;
-      empty_row(b, 0, a.Hq);
-      if (by_unit)
-        for (int u = threadIdx.x; u < units; u += 128) a.split[b * units + u] = make_int4(-1, 0, 0, 0);
-    }
-    __syncthreads();
+    n_steps = line_begin<C::STEP, D, 128>(a, units, by_unit, line, s_line);
     if (n_steps == 0) return;
-    at.b = s_b;
-    at.len = length(at.b);
-    at.nt = steps(at.len);
-    const int unit = static_cast<int>(s_at / at.nt);
-    at.t = static_cast<int>(s_at - static_cast<long long>(unit) * at.nt);
-    at.head = unit / a.row_tiles;
-    at.rt = unit - at.head * a.row_tiles;
+    at = line_at<C::STEP>(a, s_line);
   }
-  const auto next_unit = [&](PagedAt& x) {
-    x.t = 0;
-    if (++x.rt < a.row_tiles) return;
-    x.rt = 0;
-    if (++x.head < a.Hkv) return;
-    x.head = 0;
-    do x.len = length(++x.b); while (x.len == 0);
-    x.nt = steps(x.len);
-  };
 
   // ---- loads ----
   constexpr int CH = D / 8, RPI = 32 / CH;      // 16-byte pieces of a row, rows a warp covers at once
@@ -776,7 +824,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
         ++x.page;
       }
     } else {
-      next_unit(x.at);
+      next_unit<C::STEP>(a, x.at);
       x.page = page_w;
       x.off = off_w;
     }
@@ -883,7 +931,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
   clear();
   if constexpr (CLUSTER) {
     if (at.len == 0) {   // the whole cluster
-      if (rank == 0) empty_row(at.b, at.head * group + at.rt * ROWS, min(ROWS, group - at.rt * ROWS));
+      if (rank == 0) empty_row<D, 128>(a, at.b, at.head * group + at.rt * ROWS, min(ROWS, group - at.rt * ROWS));
       return;
     }
   }
@@ -1014,7 +1062,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
     // ---- the unit's end, or the stretch's ----
     const PagedAt done = at;
     if (it + 1 < n_steps) {   // the next unit's queries are on their way meanwhile
-      next_unit(at);
+      next_unit<C::STEP>(a, at);
       load_q(at);
     }
     const bool whole = first_t == 0 && done.t + 1 == done.nt;
@@ -1029,12 +1077,7 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
         if (col == 0) a.part_ml[slot] = make_float2(x.m, x.l);
       }
     });
-    if (first_t == 0 && threadIdx.x == 0 && (by_unit || !whole)) {
-      const int unit = (done.b * a.Hkv + done.head) * a.row_tiles + done.rt;
-      const long long last = g1 - 1 + (done.nt - 1 - done.t);   // the unit's last step, where it is cut
-      a.split[by_unit ? unit : static_cast<int>(blockIdx.x)] =
-          make_int4(whole ? -1 : unit, blockIdx.x, whole ? 0 : static_cast<int>(((last + 1) * blocks - 1) / total), 0);
-    }
+    if (first_t == 0 && threadIdx.x == 0) line_record(a, line, done, whole, by_unit);
     first_t = 0;
     clear();
   }

@@ -28,6 +28,7 @@
 #include "fa_fwd.cuh"
 #include "fa_fwd_persist.cuh"
 #include "fa_paged.cuh"
+#include "fa_paged_wide.cuh"
 
 namespace fab {
 
@@ -80,10 +81,16 @@ void set_smem(K kernel, int bytes) {
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+// Groups whose line paged_attn_kernel walks; the rest are paged_wide_kernel's. Time
+// of the two, 32 sequences of 4096 tokens in bf16, 4 kv heads (0.27 GB of 128-wide
+// heads, 0.13 GB of 64-wide ones), as warps / wide:
+//   17 heads: D = 128  85 / 58 us, D = 64  39 / 43;   33: 147 / 59 and 63 / 44.
+constexpr bool paged_by_warps(int D, int group) { return group <= (D == 64 ? 32 : 16); }
+
 // The paged attention's two cuts; its clusters may have 16 blocks.
 template <int D, bool BF, int ROWS>
 void set_smem_paged() {
-  set_smem(paged_attn_kernel<D, BF, ROWS, false>, PagedCfg<D>::SMEM);
+  if constexpr (paged_by_warps(D, ROWS)) set_smem(paged_attn_kernel<D, BF, ROWS, false>, PagedCfg<D>::SMEM);
   set_smem(paged_attn_kernel<D, BF, ROWS, true>, PagedCfg<D>::SMEM);
   cudaFuncSetAttribute(paged_attn_kernel<D, BF, ROWS, true>,
                        cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -109,6 +116,10 @@ void set_smem_all() {
   set_smem_paged<128, BF, 8>();
   set_smem_paged<128, BF, 16>();
   set_smem_paged<128, BF, 32>();
+  set_smem(paged_wide_kernel<64, BF, 4>, WideCfg<64>::SMEM);
+  set_smem(paged_wide_kernel<64, BF, 8>, WideCfg<64>::SMEM);
+  set_smem(paged_wide_kernel<128, BF, 4>, WideCfg<128>::SMEM);
+  set_smem(paged_wide_kernel<128, BF, 8>, WideCfg<128>::SMEM);
   set_smem(paged_join_kernel<64, BF>, 0);
   set_smem(paged_join_kernel<128, BF>, 0);
 }
@@ -307,26 +318,36 @@ struct PagedPlan {
 };
 
 PagedPlan paged_plan(int B, int Hq, int Hkv, int W, int D, int page, int sms) {
-  const int group = Hq / Hkv, step = D == 64 ? PagedCfg<64>::STEP : PagedCfg<128>::STEP;
+  const int group = Hq / Hkv;
   PagedPlan p{};
-  p.rows = group <= 8 ? 8 : group <= 16 ? 16 : 32;
-  p.row_tiles = (group + p.rows - 1) / p.rows;
-  p.units = static_cast<long long>(B) * Hkv * p.row_tiles;
-  p.most = (W * page + step - 1) / step;
+  const auto cut = [&](int rows, int step) {
+    p.rows = rows;
+    p.row_tiles = (group + rows - 1) / rows;
+    p.units = static_cast<long long>(B) * Hkv * p.row_tiles;
+    p.most = (W * page + step - 1) / step;
+  };
+  const auto line = [&](int blocks) {   // fewer where the table has no room for so many steps
+    p.blocks = static_cast<long long>(std::min<double>(blocks, static_cast<double>(p.units) * p.most));
+  };
+  cut(group <= 8 ? 8 : group <= 16 ? 16 : 32, D == 64 ? PagedCfg<64>::STEP : PagedCfg<128>::STEP);
   p.cluster = paged_cluster(p.units, p.most, sms);
-  // the line: two blocks an SM, fewer where the table has no room for so many steps
-  p.blocks = p.cluster ? p.units * p.cluster
-                       : static_cast<long long>(std::min<double>(
-                             std::min(2 * sms, kPagedMaxBlocks), static_cast<double>(p.units) * p.most));
+  if (p.cluster) {
+    p.blocks = p.units * p.cluster;
+  } else if (paged_by_warps(D, group)) {
+    line(2 * sms);
+  } else {
+    cut(128, WideCfg<64>::KEYS);
+    line(sms);
+  }
   return p;
 }
 
-// Bytes of the line's workspace: kPagedMaxBlocks records and, per block, two
-// partial results of a row tile's heads. Clusters need none.
+// Bytes of the line's workspace: a record per block and two partial results of a
+// row tile's heads. Clusters need none.
+size_t paged_rows(const PagedPlan& p, int group) { return 2 * static_cast<size_t>(std::min(group, p.rows)) * p.blocks; }
 size_t paged_workspace(const PagedPlan& p, int group, int D) {
   if (p.cluster) return 0;
-  const size_t rows = 2 * static_cast<size_t>(std::min(group, p.rows)) * kPagedMaxBlocks;
-  return kPagedMaxBlocks * sizeof(int4) + rows * (sizeof(float2) + D * sizeof(float));
+  return p.blocks * sizeof(int4) + paged_rows(p, group) * (sizeof(float2) + D * sizeof(float));
 }
 
 template <int D, bool BF, int ROWS>
@@ -336,31 +357,53 @@ int paged_attn_launch(const PagedAttnArgs& a, const PagedPlan& p, void* stream) 
   if (p.cluster)
     return launch_after(paged_attn_kernel<D, BF, ROWS, true>, "paged_attn_kernel", blocks, 128, C::SMEM,
                         p.cluster, stream, a);
-  if (int st = launch_after(paged_attn_kernel<D, BF, ROWS, false>, "paged_attn_kernel", blocks, 128, C::SMEM,
-                            0, stream, a))
-    return st;
-  if (p.most == 1) return FA_B200_OK;   // nothing is cut
-  // few units: many parts each, so 16 columns a block and 16 threads for each of them
-  const int most_cols = 8 * p.units <= p.blocks ? 16 : kJoinThreads;
-  const int cols = std::min(a.Hq / a.Hkv, ROWS) * (D / 4);
-  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel",
-                      dim3(static_cast<unsigned>(std::min(p.units, p.blocks)),
-                           (cols + most_cols - 1) / most_cols),
-                      kJoinThreads, 0, 0, stream, a, ROWS, most_cols);
+  if constexpr (paged_by_warps(D, ROWS))
+    return launch_after(paged_attn_kernel<D, BF, ROWS, false>, "paged_attn_kernel", blocks, 128, C::SMEM, 0,
+                        stream, a);
+  return FA_B200_ERR_SHAPE;   // not reached: paged_wide_launch takes these
 }
 
 template <int D, bool BF>
-int paged_attn_impl(PagedAttnArgs& a, const PagedPlan& p, void* workspace, void* stream) {
+int paged_wide_launch(const PagedAttnArgs& a, const PagedPlan& p, const Strides& sk, const Strides& sv,
+                      void* stream) {
+  int run_log2 = 4;   // the largest run of keys that divides a page and a step
+  while (run_log2 < 7 && a.page % (2 << run_log2) == 0) ++run_log2;
+  const CUtensorMapDataType dt = BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUtensorMap tk, tv;
+  if (!make_map4(&tk, a.k_cache, dt, 2, D, a.page, a.Hkv, a.P, sk, 1u << run_log2) ||
+      !make_map4(&tv, a.v_cache, dt, 2, D, a.page, a.Hkv, a.P, sv, 1u << run_log2))
+    return FA_B200_ERR_TENSOR_MAP;
+  const auto blocks = static_cast<unsigned>(p.blocks);
+  if (a.Hq / a.Hkv <= 64)
+    return launch_after(paged_wide_kernel<D, BF, 4>, "paged_wide_kernel", blocks, 192, WideCfg<D>::SMEM, 0, stream,
+                        tk, tv, a, run_log2);
+  return launch_after(paged_wide_kernel<D, BF, 8>, "paged_wide_kernel", blocks, 320, WideCfg<D>::SMEM, 0, stream,
+                      tk, tv, a, run_log2);
+}
+
+template <int D, bool BF>
+int paged_attn_impl(PagedAttnArgs& a, const PagedPlan& p, const Strides& sk, const Strides& sv, void* workspace,
+                    void* stream) {
+  const int group = a.Hq / a.Hkv;
   a.row_tiles = p.row_tiles;
   if (!p.cluster) {
-    const size_t rows = 2 * static_cast<size_t>(std::min(a.Hq / a.Hkv, p.rows)) * kPagedMaxBlocks;
     a.split = static_cast<int4*>(workspace);
-    a.part_o = reinterpret_cast<float*>(a.split + kPagedMaxBlocks);
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + rows * D);
+    a.part_o = reinterpret_cast<float*>(a.split + p.blocks);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + paged_rows(p, group) * D);
   }
-  if (p.rows == 8) return paged_attn_launch<D, BF, 8>(a, p, stream);
-  if (p.rows == 16) return paged_attn_launch<D, BF, 16>(a, p, stream);
-  return paged_attn_launch<D, BF, 32>(a, p, stream);
+  if (int st = p.rows == 8    ? paged_attn_launch<D, BF, 8>(a, p, stream)
+               : p.rows == 16 ? paged_attn_launch<D, BF, 16>(a, p, stream)
+               : p.rows == 32 ? paged_attn_launch<D, BF, 32>(a, p, stream)
+                              : paged_wide_launch<D, BF>(a, p, sk, sv, stream))
+    return st;
+  if (p.cluster || p.most == 1) return FA_B200_OK;   // nothing is cut
+  // few units: many parts each, so 16 columns a block and 16 threads for each of them
+  const int most_cols = 8 * p.units <= p.blocks ? 16 : kJoinThreads;
+  const int cols = std::min(group, p.rows) * (D / 4);
+  return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel",
+                      dim3(static_cast<unsigned>(std::min(p.units, p.blocks)),
+                           (cols + most_cols - 1) / most_cols),
+                      kJoinThreads, 0, 0, stream, a, p.rows, most_cols);
 }
 
 // An fp32 dQ is produced by the fused kernel: one pass, dQ added into the
@@ -1131,10 +1174,10 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
   if (need && (!workspace || workspace_bytes < need)) return FA_B200_ERR_WORKSPACE;
   const bool bf = dtype == FA_B200_DTYPE_BF16;
   if (D == 64)
-    return bf ? fab::paged_attn_impl<64, true>(a, plan, workspace, stream)
-              : fab::paged_attn_impl<64, false>(a, plan, workspace, stream);
-  return bf ? fab::paged_attn_impl<128, true>(a, plan, workspace, stream)
-            : fab::paged_attn_impl<128, false>(a, plan, workspace, stream);
+    return bf ? fab::paged_attn_impl<64, true>(a, plan, sk, sv, workspace, stream)
+              : fab::paged_attn_impl<64, false>(a, plan, sk, sv, workspace, stream);
+  return bf ? fab::paged_attn_impl<128, true>(a, plan, sk, sv, workspace, stream)
+            : fab::paged_attn_impl<128, false>(a, plan, sk, sv, workspace, stream);
 }
 
 size_t fa_b200_backward_workspace_bytes(int B, int Hq, int N) {

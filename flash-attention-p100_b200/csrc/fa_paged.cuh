@@ -427,9 +427,11 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // Measured: 64 ragged requests of 32/8 heads of 128 (1.0 GB of cache) 155 us, 6.45
 // TB/s or 98% of the measured copy, DRAM traffic equal to the cache's bytes, a fifth
 // of the tensor pipe; one request of 131001 tokens 85 us, 6.3 TB/s; one of 1000
-// tokens 6.0 us, a chain of dependent loads (length, page, keys). Groups of 17 to
-// 32 heads, 0.26 GB: 85 us against 52 for 16, bound by the latency of two
-// fragments' products at 8 warps an SM.
+// tokens 6.0 us, a chain of dependent loads (length, page, keys). 16 heads
+// for 32 sequences of 4096 tokens, 0.27 GB: 52 us, 5.2 TB/s. Wider groups are
+// paged_wide_kernel's, but for 17 to 32 heads where clusters take them and where D
+// is 64: 39 us for half the bytes, bound by the latency of two fragments' products at
+// 8 warps an SM.
 
 // Strides of a cache in units of 16 bytes (page, head, token): products of 32
 // bits, one instruction each, that still span 64 GB.
@@ -470,8 +472,6 @@ struct PagedCfg {
   static constexpr int MERGE = WARPS * 8 * D * 4;  // the warps' fp32 results of 8 rows
   static constexpr int SMEM = RING + MERGE;
 };
-
-constexpr int kPagedMaxBlocks = 320;  // blocks of a line at most: sizes the workspace
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

@@ -1,0 +1,421 @@
+// fa_paged_wide.cuh -- the paged cache's attention for wide groups of query heads
+// (multi-query models; paged_by_warps says which), on tcgen05.
+//
+// Such a group gives each cached byte enough work that mma.sync, at the few warps
+// that accumulators in registers allow, is slower than HBM: paged_attn_kernel takes
+// 85 us at 32 heads for a 0.27 GB cache, and reads the cache once for each 32 of
+// them. Here one block an SM walks its stretch of the same line in steps of 128
+// keys: S = Q K^T and O += P V as 128-row MMAs with O in tensor memory.
+//
+// Head h is row 32 (h % 4) + h / 4 of the tile: tensor memory gives a warp the
+// lanes of one quadrant, and a quadrant's warps one scheduler, so few heads still
+// keep all four schedulers' softmax warps busy. Up to 64 heads 4 warps do, above
+// 8. A warp has 16 of its quadrant's lanes: a thread has one head and 64 of a
+// step's keys, the thread 16 further on the other 64 (TMEM shape 16x32bx2).
+//
+//   warps 0 .. W-1  queries, softmax, the unit's end
+//   warp  W         MMA issue;  warp W + 1  TMA loads, a run of keys of one page each
+// TMEM: two buffers of 128 columns, S of a step and then its P over it, and O. S of
+// step j + 2 is issued behind the products of step j, which the tensor core finishes
+// first, so the softmax of a step waits for its S alone.
+// Weights are two 16-bit terms and lse is summed in fp32, as in paged_attn_kernel;
+// the terms' products stay apart so that an infinite value takes the first alone. Up
+// to 64 heads P's second terms are the rows 16 lanes further on and one product
+// serves both (48.0 -> 43.3 us at 32 heads, D = 64, against a product of their own).
+// Above, they are columns [64,128) of P, and their products columns [384, 384 + D).
+//
+// Measured, the sequences of paged_by_warps, for 33 / 64 / 128 heads: D = 128 59 / 62 /
+// 80 us (4.6 / 4.4 / 3.4 TB/s), D = 64 44 / 45 / 60 us. One block an SM takes a step
+// of 128 x 128 keys through K, softmax and V in turn: up to 64 heads the length of
+// that chain bounds it, not the 5 (12) tiles in flight; above, the softmax's issue.
+#pragma once
+#include "fa_fwd.cuh"
+#include "fa_paged.cuh"
+
+namespace fab {
+
+template <int D>
+struct WideCfg {
+  static constexpr int KEYS = 128;               // of a step
+  static constexpr int CH = D / 64;              // 64-column chunks of a row
+  static constexpr int TILE = 128 * D * 2;       // bytes of Q, of a step's K and of its V
+  static constexpr int SLOTS = D == 128 ? 5 : 12;  // ring: K_0, V_0, K_1, V_1, ...
+  static constexpr int OFF_RING = 2 * TILE;      // behind two Q tiles: a unit's and the next one's
+  static constexpr int OFF_BAR = OFF_RING + SLOTS * TILE;
+  // barriers: q[2], full[SLOTS], empty[SLOTS], s[2], pv[2], p[2],
+  // done; those of two are a step's by its parity, as its issue runs ahead of its use
+  static constexpr int NBAR = 2 + 2 * SLOTS + 7;
+  static constexpr int FLAGS = 32;                        // steps whose bad runs are kept
+  static constexpr int OFF_FLAGS = OFF_BAR + NBAR * 8;
+  static constexpr int SMEM = OFF_FLAGS + FLAGS * 4 + 16;
+  static_assert(SMEM + 1024 <= 232448, "shared memory over the per-block limit");
+  static constexpr uint32_t COL_O = 256, COL_O2 = 384, COLS = 512;
+};
+
+// A tile's place in the ring: 2 j is K of step j, 2 j + 1 its V.
+template <int SLOTS>
+struct RingAt {
+  int slot;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void skip(int tiles) {   // at most SLOTS
+    slot += tiles;
+    if (slot >= SLOTS) {
+      slot -= SLOTS;
+      phase ^= 1;
+    }
+  }
+};
+
+// W softmax warps: 4 for up to 64 heads of a row tile, 8 above.
+// `run_log2`: a run of 2^run_log2 keys lies in one page and is one box of tm_k, tm_v.
+template <int D, bool BF, int W>
+__global__ void __launch_bounds__(32 * (W + 2), 1)
+    paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const PagedAttnArgs a, int run_log2) {
+  using C = WideCfg<D>;
+  constexpr int SOFTMAX = 32 * W, MMA_WARP = W, TMA_WARP = W + 1;
+  constexpr float kBias = weight_bias<BF>();
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ LineShared s_line;
+  if (!smem_aligned_or_report(smem, a.err)) return;
+  const uint32_t s_q = smem_u32(smem), s_ring = s_q + C::OFF_RING;
+  const uint32_t b_q = s_q + C::OFF_BAR, b_full = b_q + 16, b_empty = b_full + 8 * C::SLOTS;
+  const uint32_t b_s = b_empty + 8 * C::SLOTS, b_pv = b_s + 16, b_p = b_pv + 16,
+                 b_done = b_p + 16;
+  int* s_bad = reinterpret_cast<int*>(smem + C::OFF_FLAGS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_bad + C::FLAGS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
+  const bool by_unit = static_cast<long long>(a.B) * units <= gridDim.x;
+  const Ctl ctl{abort_flag, a.err};
+
+  wait_for_prior_launch();
+  Line line;
+  const long long n = line_begin<C::KEYS, D, 32 * (W + 2)>(a, units, by_unit, line, s_line);
+  if (n == 0) return;
+  if (threadIdx.x == 0) {
+    mbar_init(b_q, SOFTMAX);
+    mbar_init(b_q + 8, SOFTMAX);
+    for (int s = 0; s < C::SLOTS; ++s) {
+      mbar_init(b_full + 8 * s, 1);
+      mbar_init(b_empty + 8 * s, 1);
+    }
+    mbar_init(b_s, 2);   // the products, and the issuer's word that K and its bad runs are there
+    mbar_init(b_s + 8, 2);
+    mbar_init(b_p, SOFTMAX);
+    mbar_init(b_p + 8, SOFTMAX);
+    mbar_init(b_pv, 1);
+    mbar_init(b_pv + 8, 1);
+    mbar_init(b_done, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == MMA_WARP) tmem_alloc(smem_u32(tmem_slot), C::COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  PagedAt at = line_at<C::KEYS>(a, s_line);
+  const auto advance = [&](PagedAt& x) {
+    if (++x.t == x.nt) next_unit<C::KEYS>(a, x);
+  };
+  using Ring = RingAt<C::SLOTS>;
+
+  if (warp == TMA_WARP) {
+    // ------------------------------------------------------------ loads
+    const int runs = C::KEYS >> run_log2;   // 1 to 8, one a lane
+    int id = 0, off = 0;
+    const auto look_up = [&](const PagedAt& x) {
+      const int key = x.t * C::KEYS + (lane << run_log2);
+      const int page = key / a.page;
+      off = key - page * a.page;
+      // behind the last token: a page outside the cache, which loads as zeros
+      id = lane < runs && key < x.len ? a.table[x.b * a.table_stride + page] : a.P;
+    };
+    look_up(at);
+    Ring tile{0};
+    long long issued = 0;
+    bool ok = true;
+    for (long long j = 0; j < n && ok; ++j) {
+      const bool real = lane < runs && at.t * C::KEYS + (lane << run_log2) < at.len;
+      const bool bad = real && static_cast<unsigned>(id) >= static_cast<unsigned>(a.P);
+      const int page = bad ? a.P : id, row = off, head = at.head;
+      const unsigned bad_runs = __ballot_sync(0xffffffffu, bad);
+      if (bad_runs && lane == 0) atomicCAS(a.err, 0, static_cast<int>(kErrPage));
+      if (j + 1 < n) {   // the next step's pages are on their way meanwhile
+        advance(at);
+        look_up(at);
+      }
+#pragma unroll
+      for (int kind = 0; kind < 2 && ok; ++kind) {
+        const int slot = tile.slot;
+        const uint32_t full = b_full + 8 * slot;
+        ok = lane != 0 || mbar_wait(b_empty + 8 * slot, tile.phase ^ 1, ctl, kErrTimeoutLoad);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) {
+          if (kind == 0) s_bad[j % C::FLAGS] = static_cast<int>(bad_runs);
+          mbar_arrive_expect_tx(full, C::TILE);
+        }
+        __syncwarp();
+        if (lane < runs) {
+          const uint32_t dst = s_ring + slot * C::TILE + (lane << run_log2) * 128;
+#pragma unroll
+          for (int c = 0; c < C::CH; ++c)
+            tma_load_4d(dst + c * 16384, kind ? static_cast<const void*>(&tm_v) : static_cast<const void*>(&tm_k),
+                        full, c * 64, row, head, page);
+        }
+        tile.skip(1);
+        ++issued;
+      }
+    }
+    if (!ok && lane == 0) {
+      // loads in flight land before the block leaves: the last SLOTS of them
+      const int last = static_cast<int>(issued < C::SLOTS ? issued : C::SLOTS);
+      Ring i = tile;
+      i.slot -= last;
+      if (i.slot < 0) {
+        i.slot += C::SLOTS;
+        i.phase ^= 1;
+      }
+      for (int k = 0; k < last; ++k, i.skip(1)) {
+        const uint64_t t0 = globaltimer_ns();
+        while (!mbar_try_wait(b_full + 8 * i.slot, i.phase) && globaltimer_ns() - t0 < 100000000ull) {
+        }
+      }
+    }
+  } else if (warp == MMA_WARP) {
+    // ------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      Ring k{0}, v{1};
+      const auto full = [&](const Ring& x) { return mbar_wait(b_full + 8 * x.slot, x.phase, ctl, kErrTimeoutMma); };
+      // S of the next step; `ahead` is its place, `unit` its unit of the stretch,
+      // whose Q is in buffer unit & 1
+      PagedAt ahead = at;
+      int unit = 0;
+      bool new_unit = true;
+      const auto next_s = [&](int buf) -> bool {
+        if (new_unit && !mbar_wait(b_q + 8 * (unit & 1), (unit >> 1) & 1, ctl, kErrTimeoutMma)) return false;
+        if (!full(k)) return false;
+        tc_fence_after();
+        issue_qk<D, BF>(tmem + 128 * buf, s_q + (unit & 1) * C::TILE, s_ring + k.slot * C::TILE);
+        mma_commit(b_s + 8 * buf);
+        mbar_arrive(b_s + 8 * buf);
+        mma_commit(b_empty + 8 * k.slot);
+        k.skip(2);
+        new_unit = ahead.t + 1 == ahead.nt;
+        if (new_unit) ++unit;
+        return true;
+      };
+      bool ok = next_s(0);
+      if (ok && n > 1) {
+        advance(ahead);
+        ok = next_s(1);
+      }
+      bool first = true;       // the unit's first step here: O starts over
+      for (long long j = 0; j < n && ok; ++j) {
+        ok = full(v) && mbar_wait(b_p + 8 * (j & 1), (j >> 1) & 1, ctl, kErrTimeoutMma);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t p = tmem + 128 * (j & 1);
+        issue_pv<D, BF>(tmem + C::COL_O, p, s_ring + v.slot * C::TILE, !first);
+        if (W == 8) issue_pv<D, BF>(tmem + C::COL_O2, p + 64, s_ring + v.slot * C::TILE, !first);
+        mma_commit(b_pv + 8 * (j & 1));
+        mma_commit(b_empty + 8 * v.slot);
+        v.skip(2);
+        first = at.t + 1 == at.nt;
+        if (j + 1 < n) advance(at);
+        if (j + 2 < n) {
+          advance(ahead);
+          ok = next_s(j & 1);
+        }
+      }
+      // every MMA issued above completes before tensor memory is released
+      mma_commit(b_done);
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(b_done, 0) && globaltimer_ns() - t0 < FAB_WAIT_LIMIT_NS) {
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int half = lane >> 4;
+    const int row = 32 * (warp & 3) + 16 * (warp >> 2) + (lane & 15);
+    const int head_row = 4 * (row % 32) + row / 32;   // this row's head in the tile
+    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3) + 16 * (warp >> 2)) << 16;
+    // second terms of P, from S's address, and of O
+    constexpr uint32_t kP2 = W == 4 ? 16u << 16 : 64u;
+    const uint32_t t_o = tmem + lanes + C::COL_O, t_o2 = W == 4 ? t_o + kP2 : tmem + lanes + C::COL_O2;
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
+      const bool ok = mbar_wait(bar, parity, ctl, kErrTimeoutSoftmax);
+      return static_cast<bool>(__all_sync(0xffffffffu, ok));
+    };
+    // the unit's Q tile, a row or half of one a thread; rows without a head are zero
+    const auto load_q = [&](const PagedAt& x, int buf) {
+      constexpr int PIECES = D / 8 * 128 / SOFTMAX;
+      const int qrow = threadIdx.x % 128, c0 = static_cast<int>(threadIdx.x) / 128 * PIECES;
+      const int r = x.rt * 128 + 4 * (qrow % 32) + qrow / 32;
+      const bool real = r < group && (W == 8 || qrow % 32 < 16);
+      const uint16_t* q = a.q + a.sq.at(x.b, x.head * group + (real ? r : 0), 0) + c0 * 8;
+      uint4 piece[PIECES];
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c)
+        piece[c] = real ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < PIECES; ++c)
+        st_shared_v4(s_q + buf * C::TILE + sw128_offset(qrow, c0 + c, 128), piece[c].x, piece[c].y, piece[c].z,
+                     piece[c].w);
+      fence_async_smem();
+      mbar_arrive(b_q + 8 * buf);
+    };
+    load_q(at, 0);
+    float m = -INFINITY, l = 0.f;
+    int unit = 0, first_t = at.t;
+    bool ok = true, first = true;   // first: of the unit here, whose Q is in buffer unit & 1
+    Ring v{1};
+    for (long long j = 0; j < n && ok; ++j, v.skip(2)) {
+      const long long left_here = n - j;
+      if (first && at.nt - at.t < left_here) {   // the next unit's queries
+        PagedAt x = at;
+        next_unit<C::KEYS>(a, x);
+        load_q(x, (unit + 1) & 1);
+      }
+      const uint32_t t_s = tmem + lanes + 128 * (j & 1);
+      ok = wait(b_s + 8 * (j & 1), (j >> 1) & 1);
+      // this S came behind the products of step j - 2: their phase is seen here, in
+      // order, so that later waits mean the phase they name
+      if (j >= 2) ok = ok && wait(b_pv + 8 * (j & 1), ((j >> 1) + 1) & 1);
+      if (!ok) break;
+      const unsigned bad = static_cast<unsigned>(s_bad[j % C::FLAGS]);
+      tc_fence_after();
+      uint32_t sr[64];   // keys 64 half ..
+      tmem_ld16x2_x64(t_s, sr);
+      tmem_ld_wait(sr);
+      float* s = reinterpret_cast<float*>(sr);
+      const int left = at.len - at.t * C::KEYS;   // keys of this step, if below 128
+      if (left < C::KEYS || bad) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) {
+          const int key = 64 * half + i;
+          if (key >= left || (bad >> (key >> run_log2) & 1)) s[i] = -INFINITY;
+        }
+      }
+      float top = fmaxf(s[0], s[1]);
+#pragma unroll
+      for (int i = 2; i < 64; i += 2) top = max3f(top, s[i], s[i + 1]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * a.scale;
+      float w = 1.f;
+      bool rescale = false;
+      if (first) {
+        m = top;
+      } else {
+        const bool grown = top > m + 8.f;
+        rescale = __any_sync(0xffffffffu, grown);
+        if (grown) {
+          w = ex2(m - top);   // 0 from -inf; the products so far are then 0
+          m = top;
+          l *= w;
+        }
+      }
+      const float ref = m == -INFINITY ? 0.f : kBias - m;
+      uint32_t hi[32], lo[32];   // keys 2 i, 2 i + 1 of this thread's
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const float x = ex2(fmaf(s[2 * i], a.scale, ref)), y = ex2(fmaf(s[2 * i + 1], a.scale, ref));
+        l += x + y;
+        hi[i] = pack2<BF>(x, y);
+        const float2 r = unpack2<BF>(hi[i]);
+        lo[i] = pack2<BF>(x - r.x, y - r.y);
+      }
+      __syncwarp();
+      if (rescale) {   // O is free once the products of the step before are done
+        ok = wait(b_pv + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int i = 0; i < 2 * (D / 64); ++i) {   // this thread's half of every 64 columns
+          const uint32_t col = i < D / 64 ? t_o + 64 * i : t_o2 + 64 * (i - D / 64);
+          uint32_t o[32];
+          tmem_ld16x2_x32(col, o);
+          tmem_ld_wait(o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * w);
+          tmem_st16x2_x32(col, o);
+        }
+      }
+      tmem_st16x2_x32(t_s, hi);
+      tmem_st16x2_x32(t_s + kP2, lo);
+      if (left < C::KEYS) {
+        // values behind the last token in its run: 0 weights must not meet NaN
+        ok = wait(b_full + 8 * v.slot, v.phase);
+        if (!ok) break;
+        const int end = (((left - 1) >> run_log2) + 1) << run_log2;
+        const uint32_t rows = s_ring + v.slot * C::TILE;
+        for (int i = threadIdx.x; i < (end - left) * 8 * C::CH; i += SOFTMAX) {
+          const int r = left + i / (8 * C::CH), c = i % (8 * C::CH);
+          st_shared_v4(rows + (c >> 3) * 16384 + r * 128 + ((c & 7) << 4), 0, 0, 0, 0);
+        }
+        fence_async_smem();
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(b_p + 8 * (j & 1));
+      const bool ends = at.t + 1 == at.nt;
+      if (!ends && j + 1 < n) {
+        ++at.t;
+        first = false;
+        continue;
+      }
+
+      // ---- the unit's end, or the stretch's ----
+      ok = wait(b_pv + 8 * (j & 1), (j >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const bool whole = first_t == 0 && ends;
+      const int r = at.rt * 128 + head_row;
+      PartSum part;
+      part.m = m;
+      part.l = l + __shfl_xor_sync(0xffffffffu, l, 16);
+      const long long slot = (2ll * blockIdx.x + (first_t == 0)) * min(group, 128) + head_row;
+#pragma unroll 1
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t o[32], o2[32];
+        tmem_ld16x2_x32(t_o + 64 * c, o);
+        tmem_ld16x2_x32(t_o2 + 64 * c, o2);
+        tmem_ld_wait(o);
+        tmem_ld_wait(o2);
+        if (r < group) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const auto x = [&](int e) { return add_finite(__uint_as_float(o[i + e]), __uint_as_float(o2[i + e])); };
+            const int col = 64 * c + 32 * half + i;
+            part.o = make_float4(x(0), x(1), x(2), x(3));
+            if (whole) {
+              store_part_sum<BF>(a, part, at.b, at.head * group + r, col);
+            } else {
+              *reinterpret_cast<float4*>(a.part_o + slot * D + col) = part.o;
+              if (col == 0) a.part_ml[slot] = make_float2(part.m, part.l);
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (first_t == 0 && threadIdx.x == 0) line_record(a, line, at, whole, by_unit);
+      if (j + 1 < n) next_unit<C::KEYS>(a, at);
+      ++unit;
+      first_t = 0;
+      first = true;
+      l = 0.f;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == MMA_WARP) {
+    __syncwarp();
+    tmem_dealloc(tmem, C::COLS);
+  }
+}
+
+}  // namespace fab

@@ -356,6 +356,56 @@ def test_attn_pages(cuda, ps, layout, D):
     check_attn(*s, *paged.paged_attn(*s))
 
 
+@pytest.mark.parametrize("G", [17, 32, 33, 64, 65, 128, 129, 200])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
+def test_attn_wide_groups(cuda, G, D, dtype):
+    """More units than clusters can take, groups above 16 heads: the kernel on
+    tensor memory, with lengths around its steps of 128 keys."""
+    rng = random.Random(G)
+    lens = [rng.choice([0, 1, 15, 16, 17, 127, 128, 129, 255, 256, 257, rng.randint(1, 700)]) for _ in range(300)]
+    s = scene(cuda, 300, G, 1, D, 16, lens, dtype, seed=G + D)
+    out = paged.paged_attn(*s)
+    fa_p100.check_device_errors(cuda)
+    check_attn(*s, *out)
+    again = paged.paged_attn(*s)
+    assert torch.equal(bits(out[0]), bits(again[0])) and torch.equal(out[1], again[1])
+    fa_p100.check_device_errors(cuda)
+
+
+@pytest.mark.parametrize("ps", [16, 48, 64, 80, 128, 4096])
+@pytest.mark.parametrize("layout", ["head", "row", "pair"])
+def test_attn_wide_pages(cuda, ps, layout):
+    """Page sizes and layouts in the same kernel, and table entries without a page."""
+    rng = random.Random(ps)
+    lens = [rng.randint(0, 600) for _ in range(160)]
+    s = scene(cuda, 160, 80, 2, 128, ps, lens, torch.bfloat16, layout, seed=ps)
+    check_attn(*s, *paged.paged_attn(*s))
+    fa_p100.check_device_errors(cuda)
+    table, skip = s[3], set()
+    for r in range(0, 160, 7):
+        j = rng.randrange(table.size(1))
+        table[r, j] = rng.choice([-1, s[1].size(0), 2 ** 31 - 1, -2 ** 31])
+        skip.add((r, j))
+    check_attn(*s, *paged.paged_attn(*s), skip=skip)
+    _lib.device_error(0)
+
+
+@pytest.mark.parametrize("G", [4, 16, 32, 40])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dim", [0, 1])
+def test_attn_expanded(cuda, G, D, dim):
+    """Caches that repeat one head, or one page, by a stride of 0 are only read."""
+    q, kc, vc, table, lens = scene(cuda, 160, 2 * G, 1, D, 32, [1 + 3 * i for i in range(160)],
+                                   torch.bfloat16, seed=G + D)
+    if dim == 0:   # page 0 for every page, all of it tokens
+        kc, vc = (torch.randn(1, 2, 32, D, device=cuda).to(x).expand(x.size(0), -1, -1, -1) for x in (kc, vc))
+    else:
+        kc, vc = kc.expand(-1, 2, -1, -1), vc.expand(-1, 2, -1, -1)
+    check_attn(q, kc, vc, table, lens, *paged.paged_attn(q, kc, vc, table, lens))
+    fa_p100.check_device_errors(cuda)
+
+
 @pytest.mark.parametrize("lens", [[1], [0], [16], [300], [1537], [5000], [40000], [1, 30000], [0, 0, 9000],
                                   [30000, 0, 1, 7], [2048] * 16, [777] * 100, [1] * 300,
                                   list(range(0, 2000, 13))], ids=lambda l: f"{len(l)}x{max(l)}")
@@ -385,8 +435,8 @@ def test_attn_sharp_and_flat(cuda):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["fp16", "bf16"])
-@pytest.mark.parametrize("heads", [(8, 2), (20, 2), (50, 2)], ids=lambda h: f"{h[0]}-{h[1]}")
-@pytest.mark.parametrize("B", [4, 40])
+@pytest.mark.parametrize("heads", [(8, 2), (20, 2), (50, 2), (100, 2)], ids=lambda h: f"{h[0]}-{h[1]}")
+@pytest.mark.parametrize("B", [4, 40, 400])
 def test_attn_non_finite_values(cuda, heads, dtype, B):
     """Infinities and NaN in keys and values that are seen act as in the formula;
     in another request's pages they do not act at all."""

@@ -84,7 +84,7 @@ void set_smem(K kernel, int bytes) {
 // Groups whose line paged_attn_kernel walks; the rest are paged_wide_kernel's. Time
 // of the two, 32 sequences of 4096 tokens in bf16, 4 kv heads (0.27 GB of 128-wide
 // heads, 0.13 GB of 64-wide ones), as warps / wide:
-//   17 heads: D = 128  85 / 58 us, D = 64  39 / 43;   33: 147 / 59 and 63 / 44.
+//   17 heads: D = 128  85 / 55 us, D = 64  38.5 / 40.2;   33: 147 / 57 and 63 / 41.
 constexpr bool paged_by_warps(int D, int group) { return group <= (D == 64 ? 32 : 16); }
 
 // The paged attention's two cuts; its clusters may have 16 blocks.
@@ -116,10 +116,10 @@ void set_smem_all() {
   set_smem_paged<128, BF, 8>();
   set_smem_paged<128, BF, 16>();
   set_smem_paged<128, BF, 32>();
-  set_smem(paged_wide_kernel<64, BF, 4>, WideCfg<64>::SMEM);
-  set_smem(paged_wide_kernel<64, BF, 8>, WideCfg<64>::SMEM);
-  set_smem(paged_wide_kernel<128, BF, 4>, WideCfg<128>::SMEM);
-  set_smem(paged_wide_kernel<128, BF, 8>, WideCfg<128>::SMEM);
+  set_smem(paged_wide_kernel<64, BF, 4>, WideCfg<64, 4>::SMEM);
+  set_smem(paged_wide_kernel<64, BF, 8>, WideCfg<64, 8>::SMEM);
+  set_smem(paged_wide_kernel<128, BF, 4>, WideCfg<128, 4>::SMEM);
+  set_smem(paged_wide_kernel<128, BF, 8>, WideCfg<128, 8>::SMEM);
   set_smem(paged_join_kernel<64, BF>, 0);
   set_smem(paged_join_kernel<128, BF>, 0);
 }
@@ -336,8 +336,9 @@ PagedPlan paged_plan(int B, int Hq, int Hkv, int W, int D, int page, int sms) {
   } else if (paged_by_warps(D, group)) {
     line(2 * sms);
   } else {
-    cut(128, WideCfg<64>::KEYS);
-    line(sms);
+    const bool pair = group <= 64;
+    cut(128, pair ? WideCfg<64, 4>::KEYS : WideCfg<64, 8>::KEYS);
+    line(pair ? 2 * sms : sms);
   }
   return p;
 }
@@ -366,18 +367,19 @@ int paged_attn_launch(const PagedAttnArgs& a, const PagedPlan& p, void* stream) 
 template <int D, bool BF>
 int paged_wide_launch(const PagedAttnArgs& a, const PagedPlan& p, const Strides& sk, const Strides& sv,
                       void* stream) {
+  const bool pair = a.Hq / a.Hkv <= 64;
   int run_log2 = 4;   // the largest run of keys that divides a page and a step
-  while (run_log2 < 7 && a.page % (2 << run_log2) == 0) ++run_log2;
+  while ((1 << run_log2) < (pair ? WideCfg<D, 4>::KEYS : WideCfg<D, 8>::KEYS) && a.page % (2 << run_log2) == 0) ++run_log2;
   const CUtensorMapDataType dt = BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   CUtensorMap tk, tv;
   if (!make_map4(&tk, a.k_cache, dt, 2, D, a.page, a.Hkv, a.P, sk, 1u << run_log2) ||
       !make_map4(&tv, a.v_cache, dt, 2, D, a.page, a.Hkv, a.P, sv, 1u << run_log2))
     return FA_B200_ERR_TENSOR_MAP;
   const auto blocks = static_cast<unsigned>(p.blocks);
-  if (a.Hq / a.Hkv <= 64)
-    return launch_after(paged_wide_kernel<D, BF, 4>, "paged_wide_kernel", blocks, 192, WideCfg<D>::SMEM, 0, stream,
+  if (pair)
+    return launch_after(paged_wide_kernel<D, BF, 4>, "paged_wide_kernel", blocks, 192, WideCfg<D, 4>::SMEM, 0, stream,
                         tk, tv, a, run_log2);
-  return launch_after(paged_wide_kernel<D, BF, 8>, "paged_wide_kernel", blocks, 320, WideCfg<D>::SMEM, 0, stream,
+  return launch_after(paged_wide_kernel<D, BF, 8>, "paged_wide_kernel", blocks, 320, WideCfg<D, 8>::SMEM, 0, stream,
                       tk, tv, a, run_log2);
 }
 

@@ -4,53 +4,88 @@
 // Such a group gives each cached byte enough work that mma.sync, at the few warps
 // that accumulators in registers allow, is slower than HBM: paged_attn_kernel takes
 // 85 us at 32 heads for a 0.27 GB cache, and reads the cache once for each 32 of
-// them. Here one block an SM walks its stretch of the same line in steps of 128
-// keys: S = Q K^T and O += P V as 128-row MMAs with O in tensor memory.
+// them. Here a block walks its stretch of the same line in steps of 64 or 128 keys:
+// S = Q K^T and O += P V as 128-row MMAs with O in tensor memory.
 //
-// Head h is row 32 (h % 4) + h / 4 of the tile: tensor memory gives a warp the
+// Head h is row h / 4 of quadrant h % 4 of the tile: tensor memory gives a warp the
 // lanes of one quadrant, and a quadrant's warps one scheduler, so few heads still
-// keep all four schedulers' softmax warps busy. Up to 64 heads 4 warps do, above
-// 8. A warp has 16 of its quadrant's lanes: a thread has one head and 64 of a
-// step's keys, the thread 16 further on the other 64 (TMEM shape 16x32bx2).
+// keep all four schedulers' softmax warps busy. A warp has 16 of its quadrant's
+// lanes: a thread has one head and half a step's keys, the thread 16 further on the
+// other half (TMEM shape 16x32bx2). W is the number of softmax warps:
+//
+//   W = 4, up to 64 heads: steps of 64 keys, two blocks an SM, each of half its shared
+//     and tensor memory, so that one's softmax runs beside the other's loads and
+//     products (32 heads: 59.0 -> 56.0 us against one block and 128 keys). A unit's
+//     heads take 16 lanes of each quadrant; the next unit's queries go into the other
+//     16, whose products nobody reads meanwhile.
+//   W = 8, 65 to 128 heads of a row tile: steps of 128 keys, one block, two Q tiles.
 //
 //   warps 0 .. W-1  queries, softmax, the unit's end
 //   warp  W         MMA issue;  warp W + 1  TMA loads, a run of keys of one page each
-// TMEM: two buffers of 128 columns, S of a step and then its P over it, and O. S of
+// TMEM: two buffers of KEYS columns, S of a step and then its P over it, and O. S of
 // step j + 2 is issued behind the products of step j, which the tensor core finishes
 // first, so the softmax of a step waits for its S alone.
 // Weights are two 16-bit terms and lse is summed in fp32, as in paged_attn_kernel;
-// the terms' products stay apart so that an infinite value takes the first alone. Up
-// to 64 heads P's second terms are the rows 16 lanes further on and one product
-// serves both (48.0 -> 43.3 us at 32 heads, D = 64, against a product of their own).
-// Above, they are columns [64,128) of P, and their products columns [384, 384 + D).
+// the terms' products stay apart so that an infinite value takes the first alone. At
+// W = 4 P's second terms are the quadrant's other 16 rows and one product serves both
+// (64-wide heads: 48.0 -> 43.3 us against a product of their own). At W = 8 they
+// are columns [64,128) of P, and their products columns [384, 384 + D).
 //
-// Measured, the sequences of paged_by_warps, for 33 / 64 / 128 heads: D = 128 59 / 62 /
-// 80 us (4.6 / 4.4 / 3.4 TB/s), D = 64 44 / 45 / 60 us. One block an SM takes a step
-// of 128 x 128 keys through K, softmax and V in turn: up to 64 heads the length of
-// that chain bounds it, not the 5 (12) tiles in flight; above, the softmax's issue.
+// Measured, the sequences of paged_by_warps, for 32 / 64 / 128 heads: D = 128 56 / 61 /
+// 81 us (4.8 / 4.5 / 3.4 TB/s), D = 64 40 / 42 / 60 us. About 7 us are the line's start
+// and its join; at 32 heads HBM moves the rest at 5.5 TB/s, with a third of the issue
+// slots and of the tensor pipe busy. At W = 8 the chain of one step after another
+// (S, softmax, P) bounds it: the tensor memory has no room for a second block's.
 #pragma once
 #include "fa_fwd.cuh"
 #include "fa_paged.cuh"
 
 namespace fab {
 
-template <int D>
+template <int D, int W>
 struct WideCfg {
-  static constexpr int KEYS = 128;               // of a step
+  static constexpr bool PAIR = W == 4;           // two blocks an SM
+  static constexpr int KEYS = PAIR ? 64 : 128;   // of a step
   static constexpr int CH = D / 64;              // 64-column chunks of a row
-  static constexpr int TILE = 128 * D * 2;       // bytes of Q, of a step's K and of its V
+  static constexpr int CHUNK = KEYS * 128;       // bytes of a chunk of K or V
+  static constexpr int Q = 128 * D * 2;          // bytes of 128 rows of queries
+  static constexpr int TILE = KEYS * D * 2;      // of a step's K and of its V
   static constexpr int SLOTS = D == 128 ? 5 : 12;  // ring: K_0, V_0, K_1, V_1, ...
-  static constexpr int OFF_RING = 2 * TILE;      // behind two Q tiles: a unit's and the next one's
-  static constexpr int OFF_BAR = OFF_RING + SLOTS * TILE;
-  // barriers: q[2], full[SLOTS], empty[SLOTS], s[2], pv[2], p[2],
-  // done; those of two are a step's by its parity, as its issue runs ahead of its use
-  static constexpr int NBAR = 2 + 2 * SLOTS + 7;
-  static constexpr int FLAGS = 32;                        // steps whose bad runs are kept
-  static constexpr int OFF_FLAGS = OFF_BAR + NBAR * 8;
-  static constexpr int SMEM = OFF_FLAGS + FLAGS * 4 + 16;
-  static_assert(SMEM + 1024 <= 232448, "shared memory over the per-block limit");
-  static constexpr uint32_t COL_O = 256, COL_O2 = 384, COLS = 512;
+  static constexpr int OFF_RING = PAIR ? Q : 2 * Q;   // a unit's queries and the next one's
+  static constexpr int SMEM = OFF_RING + SLOTS * TILE;
+  static_assert(SMEM + 2048 <= (PAIR ? 233472 / 2 : 233472), "shared memory over the limit");
+  static constexpr int FLAGS = 32;               // steps whose bad runs are kept
+  static constexpr uint32_t COL_O = 2 * KEYS, COL_O2 = COL_O + 128, COLS = PAIR ? 256 : 512;
 };
+
+// Barriers; those of two are a step's (q: a unit's) by its parity, as its issue runs
+// ahead of its use.
+template <int SLOTS>
+struct WideShared {
+  uint64_t q[2], full[SLOTS], empty[SLOTS], s[2], pv[2], p[2], done;
+  uint32_t tmem;
+  int abort;
+};
+
+// S (128 x KEYS) = Q (128 x D, K-major) K_step^T
+template <int D, bool BF, int KEYS>
+__device__ __forceinline__ void issue_qk_step(uint32_t d_tmem, uint32_t q_s, uint32_t k_s) {
+  constexpr uint32_t idesc = idesc_f16(128, KEYS, false, false, BF);
+  const uint64_t dq = sdesc_sw128(q_s, 16, 1024), dk = sdesc_sw128(k_s, 16, 1024);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk)
+    mma_ss(d_tmem, sdesc_add(dq, (kk >> 2) * 16384 + (kk & 3) * 32),
+           sdesc_add(dk, (kk >> 2) * KEYS * 128 + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+}
+// O (128 x D) (+)= P (128 x KEYS, pairs in tensor memory) V_step (MN-major)
+template <int D, bool BF, int KEYS>
+__device__ __forceinline__ void issue_pv_step(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_s, bool accumulate) {
+  constexpr uint32_t idesc = idesc_f16(128, D, false, true, BF);
+  const uint64_t dv = sdesc_sw128(v_s, KEYS * 128, 1024);
+#pragma unroll
+  for (int kk = 0; kk < KEYS / 16; ++kk)
+    mma_ts(d_tmem, p_tmem + kk * 8, sdesc_add(dv, kk * 2048), idesc, (accumulate || kk > 0) ? 1u : 0u);
+}
 
 // A tile's place in the ring: 2 j is K of step j, 2 j + 1 its V.
 template <int SLOTS>
@@ -66,25 +101,26 @@ struct RingAt {
   }
 };
 
-// W softmax warps: 4 for up to 64 heads of a row tile, 8 above.
+// W softmax warps: 4 for groups of up to 64 heads, 8 above.
 // `run_log2`: a run of 2^run_log2 keys lies in one page and is one box of tm_k, tm_v.
 template <int D, bool BF, int W>
-__global__ void __launch_bounds__(32 * (W + 2), 1)
+__global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
     paged_wide_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                       const PagedAttnArgs a, int run_log2) {
-  using C = WideCfg<D>;
+  using C = WideCfg<D, W>;
   constexpr int SOFTMAX = 32 * W, MMA_WARP = W, TMA_WARP = W + 1;
+  constexpr int KEYS = C::KEYS;
   constexpr float kBias = weight_bias<BF>();
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ LineShared s_line;
   if (!smem_aligned_or_report(smem, a.err)) return;
+  __shared__ WideShared<C::SLOTS> s_bar;
+  __shared__ int s_bad[C::FLAGS];
   const uint32_t s_q = smem_u32(smem), s_ring = s_q + C::OFF_RING;
-  const uint32_t b_q = s_q + C::OFF_BAR, b_full = b_q + 16, b_empty = b_full + 8 * C::SLOTS;
-  const uint32_t b_s = b_empty + 8 * C::SLOTS, b_pv = b_s + 16, b_p = b_pv + 16,
-                 b_done = b_p + 16;
-  int* s_bad = reinterpret_cast<int*>(smem + C::OFF_FLAGS);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_bad + C::FLAGS);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const uint32_t b_q = smem_u32(s_bar.q), b_full = smem_u32(s_bar.full), b_empty = smem_u32(s_bar.empty);
+  const uint32_t b_s = smem_u32(s_bar.s), b_pv = smem_u32(s_bar.pv), b_p = smem_u32(s_bar.p),
+                 b_done = smem_u32(&s_bar.done);
+  volatile int* abort_flag = &s_bar.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
   const bool by_unit = static_cast<long long>(a.B) * units <= gridDim.x;
@@ -92,7 +128,7 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
 
   wait_for_prior_launch();
   Line line;
-  const long long n = line_begin<C::KEYS, D, 32 * (W + 2)>(a, units, by_unit, line, s_line);
+  const long long n = line_begin<KEYS, D, 32 * (W + 2)>(a, units, by_unit, line, s_line);
   if (n == 0) return;
   if (threadIdx.x == 0) {
     mbar_init(b_q, SOFTMAX);
@@ -111,23 +147,23 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == MMA_WARP) tmem_alloc(smem_u32(tmem_slot), C::COLS);
+  if (warp == MMA_WARP) tmem_alloc(smem_u32(&s_bar.tmem), C::COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  PagedAt at = line_at<C::KEYS>(a, s_line);
+  const uint32_t tmem = s_bar.tmem;
+  PagedAt at = line_at<KEYS>(a, s_line);
   const auto advance = [&](PagedAt& x) {
-    if (++x.t == x.nt) next_unit<C::KEYS>(a, x);
+    if (++x.t == x.nt) next_unit<KEYS>(a, x);
   };
   using Ring = RingAt<C::SLOTS>;
 
   if (warp == TMA_WARP) {
     // ------------------------------------------------------------ loads
-    const int runs = C::KEYS >> run_log2;   // 1 to 8, one a lane
+    const int runs = KEYS >> run_log2;   // 1 to 8, one a lane
     int id = 0, off = 0;
     const auto look_up = [&](const PagedAt& x) {
-      const int key = x.t * C::KEYS + (lane << run_log2);
+      const int key = x.t * KEYS + (lane << run_log2);
       const int page = key / a.page;
       off = key - page * a.page;
       // behind the last token: a page outside the cache, which loads as zeros
@@ -138,7 +174,7 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
     long long issued = 0;
     bool ok = true;
     for (long long j = 0; j < n && ok; ++j) {
-      const bool real = lane < runs && at.t * C::KEYS + (lane << run_log2) < at.len;
+      const bool real = lane < runs && at.t * KEYS + (lane << run_log2) < at.len;
       const bool bad = real && static_cast<unsigned>(id) >= static_cast<unsigned>(a.P);
       const int page = bad ? a.P : id, row = off, head = at.head;
       const unsigned bad_runs = __ballot_sync(0xffffffffu, bad);
@@ -163,7 +199,7 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
           const uint32_t dst = s_ring + slot * C::TILE + (lane << run_log2) * 128;
 #pragma unroll
           for (int c = 0; c < C::CH; ++c)
-            tma_load_4d(dst + c * 16384, kind ? static_cast<const void*>(&tm_v) : static_cast<const void*>(&tm_k),
+            tma_load_4d(dst + c * C::CHUNK, kind ? static_cast<const void*>(&tm_v) : static_cast<const void*>(&tm_k),
                         full, c * 64, row, head, page);
         }
         tile.skip(1);
@@ -199,7 +235,8 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
         if (new_unit && !mbar_wait(b_q + 8 * (unit & 1), (unit >> 1) & 1, ctl, kErrTimeoutMma)) return false;
         if (!full(k)) return false;
         tc_fence_after();
-        issue_qk<D, BF>(tmem + 128 * buf, s_q + (unit & 1) * C::TILE, s_ring + k.slot * C::TILE);
+        issue_qk_step<D, BF, KEYS>(tmem + KEYS * buf, C::PAIR ? s_q : s_q + (unit & 1) * C::Q,
+                                   s_ring + k.slot * C::TILE);
         mma_commit(b_s + 8 * buf);
         mbar_arrive(b_s + 8 * buf);
         mma_commit(b_empty + 8 * k.slot);
@@ -218,9 +255,9 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
         ok = full(v) && mbar_wait(b_p + 8 * (j & 1), (j >> 1) & 1, ctl, kErrTimeoutMma);
         if (!ok) break;
         tc_fence_after();
-        const uint32_t p = tmem + 128 * (j & 1);
-        issue_pv<D, BF>(tmem + C::COL_O, p, s_ring + v.slot * C::TILE, !first);
-        if (W == 8) issue_pv<D, BF>(tmem + C::COL_O2, p + 64, s_ring + v.slot * C::TILE, !first);
+        const uint32_t p = tmem + KEYS * (j & 1);
+        issue_pv_step<D, BF, KEYS>(tmem + C::COL_O, p, s_ring + v.slot * C::TILE, !first);
+        if (!C::PAIR) issue_pv_step<D, BF, KEYS>(tmem + C::COL_O2, p + KEYS / 2, s_ring + v.slot * C::TILE, !first);
         mma_commit(b_pv + 8 * (j & 1));
         mma_commit(b_empty + 8 * v.slot);
         v.skip(2);
@@ -239,32 +276,31 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
     }
   } else {
     // ------------------------------------------------------------ softmax
+    constexpr int PER = KEYS / 2;   // keys a thread
     const int half = lane >> 4;
-    const int row = 32 * (warp & 3) + 16 * (warp >> 2) + (lane & 15);
-    const int head_row = 4 * (row % 32) + row / 32;   // this row's head in the tile
-    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3) + 16 * (warp >> 2)) << 16;
-    // second terms of P, from S's address, and of O
-    constexpr uint32_t kP2 = W == 4 ? 16u << 16 : 64u;
-    const uint32_t t_o = tmem + lanes + C::COL_O, t_o2 = W == 4 ? t_o + kP2 : tmem + lanes + C::COL_O2;
+    const int head_row = 4 * (16 * (warp >> 2) + (lane & 15)) + (warp & 3);   // this thread's head in the tile
+    const uint32_t quad = tmem + (static_cast<uint32_t>(32 * (warp & 3) + 16 * (warp >> 2)) << 16);
     const auto wait = [&](uint32_t bar, uint32_t parity) {
       const bool ok = mbar_wait(bar, parity, ctl, kErrTimeoutSoftmax);
       return static_cast<bool>(__all_sync(0xffffffffu, ok));
     };
-    // the unit's Q tile, a row or half of one a thread; rows without a head are zero
+    // a unit's queries, half a row a thread; rows without a head are zero
     const auto load_q = [&](const PagedAt& x, int buf) {
-      constexpr int PIECES = D / 8 * 128 / SOFTMAX;
-      const int qrow = threadIdx.x % 128, c0 = static_cast<int>(threadIdx.x) / 128 * PIECES;
-      const int r = x.rt * 128 + 4 * (qrow % 32) + qrow / 32;
-      const bool real = r < group && (W == 8 || qrow % 32 < 16);
+      constexpr int HEADS = 16 * W, PIECES = D / 16;
+      const int i = threadIdx.x % HEADS, c0 = static_cast<int>(threadIdx.x) / HEADS * PIECES;
+      const int quadrant = i / (HEADS / 4), at_row = i % (HEADS / 4);
+      const int r = x.rt * 128 + 4 * at_row + quadrant;
+      const bool real = r < group;
       const uint16_t* q = a.q + a.sq.at(x.b, x.head * group + (real ? r : 0), 0) + c0 * 8;
       uint4 piece[PIECES];
 #pragma unroll
       for (int c = 0; c < PIECES; ++c)
         piece[c] = real ? *reinterpret_cast<const uint4*>(q + c * 8) : make_uint4(0, 0, 0, 0);
+      const int row = 32 * quadrant + (C::PAIR ? 16 * buf : 0) + at_row;
+      const uint32_t tile = C::PAIR ? s_q : s_q + buf * C::Q;
 #pragma unroll
       for (int c = 0; c < PIECES; ++c)
-        st_shared_v4(s_q + buf * C::TILE + sw128_offset(qrow, c0 + c, 128), piece[c].x, piece[c].y, piece[c].z,
-                     piece[c].w);
+        st_shared_v4(tile + sw128_offset(row, c0 + c, 128), piece[c].x, piece[c].y, piece[c].z, piece[c].w);
       fence_async_smem();
       mbar_arrive(b_q + 8 * buf);
     };
@@ -277,10 +313,13 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
       const long long left_here = n - j;
       if (first && at.nt - at.t < left_here) {   // the next unit's queries
         PagedAt x = at;
-        next_unit<C::KEYS>(a, x);
+        next_unit<KEYS>(a, x);
         load_q(x, (unit + 1) & 1);
       }
-      const uint32_t t_s = tmem + lanes + 128 * (j & 1);
+      // a pair's units take the two halves of each quadrant's lanes in turn
+      const uint32_t t_hi = C::PAIR ? quad + ((unit & 1) << 20) : quad, t_lo = C::PAIR ? t_hi ^ (1u << 20) : quad;
+      const uint32_t t_s = t_hi + KEYS * (j & 1), t_p2 = C::PAIR ? t_lo + KEYS * (j & 1) : t_s + KEYS / 2;
+      const uint32_t t_o = t_hi + C::COL_O, t_o2 = t_lo + (C::PAIR ? C::COL_O : C::COL_O2);
       ok = wait(b_s + 8 * (j & 1), (j >> 1) & 1);
       // this S came behind the products of step j - 2: their phase is seen here, in
       // order, so that later waits mean the phase they name
@@ -288,21 +327,22 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
       if (!ok) break;
       const unsigned bad = static_cast<unsigned>(s_bad[j % C::FLAGS]);
       tc_fence_after();
-      uint32_t sr[64];   // keys 64 half ..
-      tmem_ld16x2_x64(t_s, sr);
+      uint32_t sr[PER];   // keys PER half ..
+      if constexpr (PER == 64) tmem_ld16x2_x64(t_s, sr);
+      else tmem_ld16x2_x32(t_s, sr);
       tmem_ld_wait(sr);
       float* s = reinterpret_cast<float*>(sr);
-      const int left = at.len - at.t * C::KEYS;   // keys of this step, if below 128
-      if (left < C::KEYS || bad) {
+      const int left = at.len - at.t * KEYS;   // keys of this step, if below KEYS
+      if (left < KEYS || bad) {
 #pragma unroll
-        for (int i = 0; i < 64; ++i) {
-          const int key = 64 * half + i;
+        for (int i = 0; i < PER; ++i) {
+          const int key = PER * half + i;
           if (key >= left || (bad >> (key >> run_log2) & 1)) s[i] = -INFINITY;
         }
       }
       float top = fmaxf(s[0], s[1]);
 #pragma unroll
-      for (int i = 2; i < 64; i += 2) top = max3f(top, s[i], s[i + 1]);
+      for (int i = 2; i < PER; i += 2) top = max3f(top, s[i], s[i + 1]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16)) * a.scale;
       float w = 1.f;
       bool rescale = false;
@@ -318,9 +358,9 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
         }
       }
       const float ref = m == -INFINITY ? 0.f : kBias - m;
-      uint32_t hi[32], lo[32];   // keys 2 i, 2 i + 1 of this thread's
+      uint32_t hi[PER / 2], lo[PER / 2];   // keys 2 i, 2 i + 1 of this thread's
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
+      for (int i = 0; i < PER / 2; ++i) {
         const float x = ex2(fmaf(s[2 * i], a.scale, ref)), y = ex2(fmaf(s[2 * i + 1], a.scale, ref));
         l += x + y;
         hi[i] = pack2<BF>(x, y);
@@ -343,9 +383,14 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
           tmem_st16x2_x32(col, o);
         }
       }
-      tmem_st16x2_x32(t_s, hi);
-      tmem_st16x2_x32(t_s + kP2, lo);
-      if (left < C::KEYS) {
+      if constexpr (PER == 64) {
+        tmem_st16x2_x32(t_s, hi);
+        tmem_st16x2_x32(t_p2, lo);
+      } else {
+        tmem_st16x2_x16(t_s, hi);
+        tmem_st16x2_x16(t_p2, lo);
+      }
+      if (left < KEYS) {
         // values behind the last token in its run: 0 weights must not meet NaN
         ok = wait(b_full + 8 * v.slot, v.phase);
         if (!ok) break;
@@ -353,7 +398,7 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
         const uint32_t rows = s_ring + v.slot * C::TILE;
         for (int i = threadIdx.x; i < (end - left) * 8 * C::CH; i += SOFTMAX) {
           const int r = left + i / (8 * C::CH), c = i % (8 * C::CH);
-          st_shared_v4(rows + (c >> 3) * 16384 + r * 128 + ((c & 7) << 4), 0, 0, 0, 0);
+          st_shared_v4(rows + (c >> 3) * C::CHUNK + r * 128 + ((c & 7) << 4), 0, 0, 0, 0);
         }
         fence_async_smem();
       }
@@ -401,7 +446,7 @@ __global__ void __launch_bounds__(32 * (W + 2), 1)
         __syncwarp();
       }
       if (first_t == 0 && threadIdx.x == 0) line_record(a, line, at, whole, by_unit);
-      if (j + 1 < n) next_unit<C::KEYS>(a, at);
+      if (j + 1 < n) next_unit<KEYS>(a, at);
       ++unit;
       first_t = 0;
       first = true;

@@ -114,7 +114,7 @@ def build_binding(force=False):
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
            f"-I{home}/include", f"-I{home}/include/torch/csrc/api/include",
            f"-I{sysconfig.get_path('include')}", f"-I{cuda}/include", BINDING_SOURCE, "-o", tmp,
-           f"-L{home}/lib", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+           f"-L{home}/lib", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("g++ failed building _fa_paged.so:\n" + res.stdout + res.stderr)

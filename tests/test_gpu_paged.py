@@ -391,6 +391,32 @@ def test_attn_wide_pages(cuda, ps, layout):
     _lib.device_error(0)
 
 
+def test_attn_outputs(cuda):
+    """o and lse share an allocation, but neither's values nor its graph the other's;
+    the table calls' outputs likewise."""
+    s = scene(cuda, 3, 8, 2, 64, 16, [5, 0, 40], torch.float16)
+    o, lse = paged.paged_attn(*s)
+    o0, lse0 = o.clone(), lse.clone()
+    assert o.is_contiguous() and lse.is_contiguous() and not o.requires_grad and not lse.requires_grad
+    w = torch.ones(64, device=cuda, requires_grad=True)
+    (o.float() * w).sum().backward()
+    torch.testing.assert_close(w.grad, o0.float().sum((0, 1)))
+    lse.fill_(7.0)
+    assert torch.equal(o, o0)
+    o.zero_()
+    assert (lse == 7.0).all()
+    with torch.inference_mode():
+        o, lse = paged.paged_attn(*s)
+        assert o.is_inference() and torch.equal(o, o0) and torch.equal(lse, lse0)
+    lens, free = i32([5, 0, 40], cuda), i32(list(range(9)), cuda)
+    out = paged.paged_extend(i32([1, 2, 0], cuda), lens, s[3].clone(), free, i32([9], cuda), 16, 3)
+    kept = [x.clone() for x in out]
+    for i, x in enumerate(out):
+        x.fill_(99)
+        for y, k in zip(out[i + 1:], kept[i + 1:]):
+            assert torch.equal(y, k)
+
+
 @pytest.mark.parametrize("G", [4, 16, 32, 40])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("dim", [0, 1])

@@ -81,16 +81,16 @@ void set_smem(K kernel, int bytes) {
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
-// Groups whose line paged_attn_kernel walks; the rest are paged_wide_kernel's. Time
-// of the two, 32 sequences of 4096 tokens in bf16, 4 kv heads (0.27 GB of 128-wide
-// heads, 0.13 GB of 64-wide ones), as warps / wide:
-//   17 heads: D = 128  85 / 55 us, D = 64  38.5 / 40.2;   33: 147 / 57 and 63 / 41.
-constexpr bool paged_by_warps(int D, int group) { return group <= (D == 64 ? 32 : 16); }
+// Heads of a group up to which paged_attn_kernel walks the line; wider ones are
+// paged_wide_kernel's. Time of the two, 32 sequences of 4096 tokens in bf16, 4 kv heads
+// (0.27 GB of 128-wide heads, 0.13 GB of 64-wide ones), in us, of 128 / of 64:
+//   17 heads 85 / 38.5 against 53 / 38.6, 33 heads 147 / 63 against 55 / 39.
+constexpr int kPagedWarpHeads = 16;
 
 // The paged attention's two cuts; its clusters may have 16 blocks.
 template <int D, bool BF, int ROWS>
 void set_smem_paged() {
-  if constexpr (paged_by_warps(D, ROWS)) set_smem(paged_attn_kernel<D, BF, ROWS, false>, PagedCfg<D>::SMEM);
+  if constexpr (ROWS <= kPagedWarpHeads) set_smem(paged_attn_kernel<D, BF, ROWS, false>, PagedCfg<D>::SMEM);
   set_smem(paged_attn_kernel<D, BF, ROWS, true>, PagedCfg<D>::SMEM);
   cudaFuncSetAttribute(paged_attn_kernel<D, BF, ROWS, true>,
                        cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -333,7 +333,7 @@ PagedPlan paged_plan(int B, int Hq, int Hkv, int W, int D, int page, int sms) {
   p.cluster = paged_cluster(p.units, p.most, sms);
   if (p.cluster) {
     p.blocks = p.units * p.cluster;
-  } else if (paged_by_warps(D, group)) {
+  } else if (group <= kPagedWarpHeads) {
     line(2 * sms);
   } else {
     const bool pair = group <= 64;
@@ -358,7 +358,7 @@ int paged_attn_launch(const PagedAttnArgs& a, const PagedPlan& p, void* stream) 
   if (p.cluster)
     return launch_after(paged_attn_kernel<D, BF, ROWS, true>, "paged_attn_kernel", blocks, 128, C::SMEM,
                         p.cluster, stream, a);
-  if constexpr (paged_by_warps(D, ROWS))
+  if constexpr (ROWS <= kPagedWarpHeads)
     return launch_after(paged_attn_kernel<D, BF, ROWS, false>, "paged_attn_kernel", blocks, 128, C::SMEM, 0,
                         stream, a);
   return FA_B200_ERR_SHAPE;   // not reached: paged_wide_launch takes these

@@ -428,10 +428,9 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // TB/s or 98% of the measured copy, DRAM traffic equal to the cache's bytes, a fifth
 // of the tensor pipe; one request of 131001 tokens 85 us, 6.3 TB/s; one of 1000
 // tokens 6.0 us, a chain of dependent loads (length, page, keys). 16 heads
-// for 32 sequences of 4096 tokens, 0.27 GB: 52 us, 5.2 TB/s. Wider groups are
-// paged_wide_kernel's, but for 17 to 32 heads where clusters take them and where D
-// is 64: 39 us for half the bytes, bound by the latency of two fragments' products at
-// 8 warps an SM.
+// for 32 sequences of 4096 tokens, 0.27 GB: 52 us, 5.2 TB/s. Wider groups'
+// line is paged_wide_kernel's: two fragments' products at 8 warps an SM are bound by
+// their latency, 85 us at 32 heads. Clusters take them here, up to 32 heads a tile.
 
 // Strides of a cache in units of 16 bytes (page, head, token): products of 32
 // bits, one instruction each, that still span 64 GB.

@@ -1,5 +1,5 @@
 // fa_paged_wide.cuh -- the paged cache's attention for wide groups of query heads
-// (multi-query models; paged_by_warps says which), on tcgen05.
+// (multi-query models; kPagedWarpHeads says which), on tcgen05.
 //
 // Such a group gives each cached byte enough work that mma.sync, at the few warps
 // that accumulators in registers allow, is slower than HBM: paged_attn_kernel takes
@@ -31,8 +31,8 @@
 // (64-wide heads: 48.0 -> 43.3 us against a product of their own). At W = 8 they
 // are columns [64,128) of P, and their products columns [384, 384 + D).
 //
-// Measured, the sequences of paged_by_warps, for 32 / 64 / 128 heads: D = 128 56 / 61 /
-// 81 us (4.8 / 4.5 / 3.4 TB/s), D = 64 40 / 42 / 60 us. About 7 us are the line's start
+// Measured, the sequences of kPagedWarpHeads, for 32 / 64 / 128 heads: D = 128 55 / 60 /
+// 79 us (4.9 / 4.5 / 3.5 TB/s), D = 64 39 / 41 / 56 us. About 7 us are the line's start
 // and its join; at 32 heads HBM moves the rest at 5.5 TB/s, with a third of the issue
 // slots and of the tensor pipe busy. At W = 8 the chain of one step after another
 // (S, softmax, P) bounds it: the tensor memory has no room for a second block's.
@@ -59,32 +59,69 @@ struct WideCfg {
 };
 
 // Barriers; those of two are a step's (q: a unit's) by its parity, as its issue runs
-// ahead of its use.
+// ahead of its use. S of step j + 1 comes behind the products of step j - 1 and stands
+// for them, so those have barriers of their own only for the last step but one (pv)
+// and where a unit or the stretch ends (end).
 template <int SLOTS>
 struct WideShared {
-  uint64_t q[2], full[SLOTS], empty[SLOTS], s[2], pv[2], p[2], done;
+  uint64_t q[2], full[SLOTS], empty[SLOTS], s[2], p[2], pv, end, done;
   uint32_t tmem;
   int abort;
 };
 
+// The MMA warp stays whole: every lane runs its loop with the same values, and only
+// the elected lane's instructions take effect, so that descriptors are computed in
+// uniform registers. From inside a branch of one lane each MMA took 70 to 95 cycles to
+// issue, whatever its size (64-wide heads, 128 of them: 60.2 -> 56.7 us).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t lead;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(lead));
+  return lead;
+}
+__device__ __forceinline__ void mma_ss_lead(uint32_t lead, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts_lead(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+
 // S (128 x KEYS) = Q (128 x D, K-major) K_step^T
 template <int D, bool BF, int KEYS>
-__device__ __forceinline__ void issue_qk_step(uint32_t d_tmem, uint32_t q_s, uint32_t k_s) {
+__device__ __forceinline__ void issue_qk_step(uint32_t lead, uint32_t d_tmem, uint32_t q_s, uint32_t k_s) {
   constexpr uint32_t idesc = idesc_f16(128, KEYS, false, false, BF);
   const uint64_t dq = sdesc_sw128(q_s, 16, 1024), dk = sdesc_sw128(k_s, 16, 1024);
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk)
-    mma_ss(d_tmem, sdesc_add(dq, (kk >> 2) * 16384 + (kk & 3) * 32),
-           sdesc_add(dk, (kk >> 2) * KEYS * 128 + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+    mma_ss_lead(lead, d_tmem, sdesc_add(dq, (kk >> 2) * 16384 + (kk & 3) * 32),
+                sdesc_add(dk, (kk >> 2) * KEYS * 128 + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
 }
 // O (128 x D) (+)= P (128 x KEYS, pairs in tensor memory) V_step (MN-major)
 template <int D, bool BF, int KEYS>
-__device__ __forceinline__ void issue_pv_step(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_s, bool accumulate) {
+__device__ __forceinline__ void issue_pv_step(uint32_t lead, uint32_t d_tmem, uint32_t p_tmem, uint32_t v_s,
+                                              bool accumulate) {
   constexpr uint32_t idesc = idesc_f16(128, D, false, true, BF);
   const uint64_t dv = sdesc_sw128(v_s, KEYS * 128, 1024);
 #pragma unroll
   for (int kk = 0; kk < KEYS / 16; ++kk)
-    mma_ts(d_tmem, p_tmem + kk * 8, sdesc_add(dv, kk * 2048), idesc, (accumulate || kk > 0) ? 1u : 0u);
+    mma_ts_lead(lead, d_tmem, p_tmem + kk * 8, sdesc_add(dv, kk * 2048), idesc, (accumulate || kk > 0) ? 1u : 0u);
 }
 
 // A tile's place in the ring: 2 j is K of step j, 2 j + 1 its V.
@@ -118,8 +155,8 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
   __shared__ int s_bad[C::FLAGS];
   const uint32_t s_q = smem_u32(smem), s_ring = s_q + C::OFF_RING;
   const uint32_t b_q = smem_u32(s_bar.q), b_full = smem_u32(s_bar.full), b_empty = smem_u32(s_bar.empty);
-  const uint32_t b_s = smem_u32(s_bar.s), b_pv = smem_u32(s_bar.pv), b_p = smem_u32(s_bar.p),
-                 b_done = smem_u32(&s_bar.done);
+  const uint32_t b_s = smem_u32(s_bar.s), b_p = smem_u32(s_bar.p), b_pv = smem_u32(&s_bar.pv),
+                 b_end = smem_u32(&s_bar.end), b_done = smem_u32(&s_bar.done);
   volatile int* abort_flag = &s_bar.abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.Hq / a.Hkv, units = a.Hkv * a.row_tiles;
@@ -139,10 +176,10 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
     }
     mbar_init(b_s, 2);   // the products, and the issuer's word that K and its bad runs are there
     mbar_init(b_s + 8, 2);
-    mbar_init(b_p, SOFTMAX);
-    mbar_init(b_p + 8, SOFTMAX);
+    mbar_init(b_p, W);
+    mbar_init(b_p + 8, W);
     mbar_init(b_pv, 1);
-    mbar_init(b_pv + 8, 1);
+    mbar_init(b_end, 1);
     mbar_init(b_done, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -223,56 +260,65 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
     }
   } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      Ring k{0}, v{1};
-      const auto full = [&](const Ring& x) { return mbar_wait(b_full + 8 * x.slot, x.phase, ctl, kErrTimeoutMma); };
-      // S of the next step; `ahead` is its place, `unit` its unit of the stretch,
-      // whose Q is in buffer unit & 1
-      PagedAt ahead = at;
-      int unit = 0;
-      bool new_unit = true;
-      const auto next_s = [&](int buf) -> bool {
-        if (new_unit && !mbar_wait(b_q + 8 * (unit & 1), (unit >> 1) & 1, ctl, kErrTimeoutMma)) return false;
-        if (!full(k)) return false;
-        tc_fence_after();
-        issue_qk_step<D, BF, KEYS>(tmem + KEYS * buf, C::PAIR ? s_q : s_q + (unit & 1) * C::Q,
-                                   s_ring + k.slot * C::TILE);
-        mma_commit(b_s + 8 * buf);
-        mbar_arrive(b_s + 8 * buf);
-        mma_commit(b_empty + 8 * k.slot);
-        k.skip(2);
-        new_unit = ahead.t + 1 == ahead.nt;
-        if (new_unit) ++unit;
-        return true;
-      };
-      bool ok = next_s(0);
-      if (ok && n > 1) {
+    __syncwarp();
+    const uint32_t lead = elect_one(), tmem0 = __shfl_sync(0xffffffffu, tmem, 0);
+    const long long steps = __shfl_sync(0xffffffffu, n, 0);
+    const auto wait = [&](uint32_t bar, uint32_t parity) {
+      const bool ok = mbar_wait(bar, parity, ctl, kErrTimeoutMma);
+      return static_cast<bool>(__all_sync(0xffffffffu, ok));
+    };
+    const auto commit = [&](uint32_t bar) {
+      if (lead) mma_commit(bar);
+    };
+    Ring k{0}, v{1};
+    // S of the next step; `ahead` is its place, `unit` its unit of the stretch,
+    // whose Q is in buffer unit & 1
+    PagedAt ahead = at;
+    int unit = 0;
+    bool new_unit = true;
+    const auto next_s = [&](int buf) -> bool {
+      if (new_unit && !wait(b_q + 8 * (unit & 1), (unit >> 1) & 1)) return false;
+      if (!wait(b_full + 8 * k.slot, k.phase)) return false;
+      tc_fence_after();
+      issue_qk_step<D, BF, KEYS>(lead, tmem0 + KEYS * buf, C::PAIR ? s_q : s_q + (unit & 1) * C::Q,
+                                 s_ring + k.slot * C::TILE);
+      commit(b_s + 8 * buf);
+      if (lead) mbar_arrive(b_s + 8 * buf);
+      commit(b_empty + 8 * k.slot);
+      k.skip(2);
+      new_unit = __any_sync(0xffffffffu, ahead.t + 1 == ahead.nt);
+      if (new_unit) ++unit;
+      return true;
+    };
+    bool ok = next_s(0);
+    if (ok && steps > 1) {
+      advance(ahead);
+      ok = next_s(1);
+    }
+    bool first = true;       // the unit's first step here: O starts over
+    for (long long j = 0; j < steps && ok; ++j) {
+      ok = wait(b_full + 8 * v.slot, v.phase) && wait(b_p + 8 * (j & 1), (j >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t p = tmem0 + KEYS * (j & 1);
+      issue_pv_step<D, BF, KEYS>(lead, tmem0 + C::COL_O, p, s_ring + v.slot * C::TILE, !first);
+      if (!C::PAIR)
+        issue_pv_step<D, BF, KEYS>(lead, tmem0 + C::COL_O2, p + KEYS / 2, s_ring + v.slot * C::TILE, !first);
+      first = __any_sync(0xffffffffu, at.t + 1 == at.nt);
+      if (j + 2 == steps) commit(b_pv);
+      if (first || j + 1 == steps) commit(b_end);
+      commit(b_empty + 8 * v.slot);
+      v.skip(2);
+      if (j + 1 < steps) advance(at);
+      if (j + 2 < steps) {
         advance(ahead);
-        ok = next_s(1);
+        ok = next_s(j & 1);
       }
-      bool first = true;       // the unit's first step here: O starts over
-      for (long long j = 0; j < n && ok; ++j) {
-        ok = full(v) && mbar_wait(b_p + 8 * (j & 1), (j >> 1) & 1, ctl, kErrTimeoutMma);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t p = tmem + KEYS * (j & 1);
-        issue_pv_step<D, BF, KEYS>(tmem + C::COL_O, p, s_ring + v.slot * C::TILE, !first);
-        if (!C::PAIR) issue_pv_step<D, BF, KEYS>(tmem + C::COL_O2, p + KEYS / 2, s_ring + v.slot * C::TILE, !first);
-        mma_commit(b_pv + 8 * (j & 1));
-        mma_commit(b_empty + 8 * v.slot);
-        v.skip(2);
-        first = at.t + 1 == at.nt;
-        if (j + 1 < n) advance(at);
-        if (j + 2 < n) {
-          advance(ahead);
-          ok = next_s(j & 1);
-        }
-      }
-      // every MMA issued above completes before tensor memory is released
-      mma_commit(b_done);
-      const uint64_t t0 = globaltimer_ns();
-      while (!mbar_try_wait(b_done, 0) && globaltimer_ns() - t0 < FAB_WAIT_LIMIT_NS) {
-      }
+    }
+    // every MMA issued above completes before tensor memory is released
+    commit(b_done);
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(b_done, 0) && globaltimer_ns() - t0 < FAB_WAIT_LIMIT_NS) {
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -321,9 +367,6 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
       const uint32_t t_s = t_hi + KEYS * (j & 1), t_p2 = C::PAIR ? t_lo + KEYS * (j & 1) : t_s + KEYS / 2;
       const uint32_t t_o = t_hi + C::COL_O, t_o2 = t_lo + (C::PAIR ? C::COL_O : C::COL_O2);
       ok = wait(b_s + 8 * (j & 1), (j >> 1) & 1);
-      // this S came behind the products of step j - 2: their phase is seen here, in
-      // order, so that later waits mean the phase they name
-      if (j >= 2) ok = ok && wait(b_pv + 8 * (j & 1), ((j >> 1) + 1) & 1);
       if (!ok) break;
       const unsigned bad = static_cast<unsigned>(s_bad[j % C::FLAGS]);
       tc_fence_after();
@@ -369,7 +412,7 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
       }
       __syncwarp();
       if (rescale) {   // O is free once the products of the step before are done
-        ok = wait(b_pv + 8 * ((j - 1) & 1), ((j - 1) >> 1) & 1);
+        ok = j + 1 < n ? wait(b_s + 8 * ((j + 1) & 1), ((j + 1) >> 1) & 1) : wait(b_pv, 0);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
@@ -404,7 +447,8 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
       }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(b_p + 8 * (j & 1));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b_p + 8 * (j & 1));
       const bool ends = at.t + 1 == at.nt;
       if (!ends && j + 1 < n) {
         ++at.t;
@@ -413,7 +457,7 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
       }
 
       // ---- the unit's end, or the stretch's ----
-      ok = wait(b_pv + 8 * (j & 1), (j >> 1) & 1);
+      ok = wait(b_end, unit & 1);
       if (!ok) break;
       tc_fence_after();
       const bool whole = first_t == 0 && ends;

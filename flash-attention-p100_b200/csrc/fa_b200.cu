@@ -84,7 +84,7 @@ void set_smem(K kernel, int bytes) {
 // Heads of a group up to which paged_attn_kernel walks the line; wider ones are
 // paged_wide_kernel's. Time of the two, 32 sequences of 4096 tokens in bf16, 4 kv heads
 // (0.27 GB of 128-wide heads, 0.13 GB of 64-wide ones), in us, of 128 / of 64:
-//   17 heads 85 / 38.5 against 53 / 38.6, 33 heads 147 / 63 against 55 / 39.
+//   17 heads 85 / 38.5 against 53 / 37.8, 33 heads 147 / 63 against 55 / 38.4.
 constexpr int kPagedWarpHeads = 16;
 
 // The paged attention's two cuts; its clusters may have 16 blocks.

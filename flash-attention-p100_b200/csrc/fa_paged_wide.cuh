@@ -32,8 +32,8 @@
 // are columns [64,128) of P, and their products columns [384, 384 + D).
 //
 // Measured, the sequences of kPagedWarpHeads, for 32 / 64 / 128 heads: D = 128 55 / 60 /
-// 79 us (4.9 / 4.5 / 3.5 TB/s), D = 64 39 / 41 / 56 us. About 7 us are the line's start
-// and its join; at 32 heads HBM moves the rest at 5.5 TB/s, with a third of the issue
+// 79 us (4.9 / 4.5 / 3.5 TB/s), D = 64 38 / 40 / 55 us. About 7 us are the line's start
+// and its join; at 32 heads HBM moves the rest at 5.6 TB/s, with a third of the issue
 // slots and of the tensor pipe busy. At W = 8 the chain of one step after another
 // (S, softmax, P) bounds it: the tensor memory has no room for a second block's.
 #pragma once
@@ -402,14 +402,20 @@ __global__ void __launch_bounds__(32 * (W + 2), WideCfg<D, W>::PAIR ? 2 : 1)
       }
       const float ref = m == -INFINITY ? 0.f : kBias - m;
       uint32_t hi[PER / 2], lo[PER / 2];   // keys 2 i, 2 i + 1 of this thread's
+      const uint64_t scale2 = f32x2(a.scale, a.scale), ref2 = f32x2(ref, ref), minus = f32x2(-1.f, -1.f);
+      uint64_t sum[2] = {f32x2(0.f, 0.f), f32x2(0.f, 0.f)};
 #pragma unroll
       for (int i = 0; i < PER / 2; ++i) {
-        const float x = ex2(fmaf(s[2 * i], a.scale, ref)), y = ex2(fmaf(s[2 * i + 1], a.scale, ref));
-        l += x + y;
+        const float2 e = f32x2_split(fma_x2(f32x2(s[2 * i], s[2 * i + 1]), scale2, ref2));
+        const float x = ex2(e.x), y = ex2(e.y);
+        const uint64_t xy = f32x2(x, y);
+        sum[i & 1] = add_x2(sum[i & 1], xy);
         hi[i] = pack2<BF>(x, y);
-        const float2 r = unpack2<BF>(hi[i]);
-        lo[i] = pack2<BF>(x - r.x, y - r.y);
+        const float2 r = unpack2<BF>(hi[i]), rest = f32x2_split(fma_x2(f32x2(r.x, r.y), minus, xy));
+        lo[i] = pack2<BF>(rest.x, rest.y);
       }
+      const float2 both = f32x2_split(add_x2(sum[0], sum[1]));
+      l += both.x + both.y;
       __syncwarp();
       if (rescale) {   // O is free once the products of the step before are done
         ok = j + 1 < n ? wait(b_s + 8 * ((j + 1) & 1), ((j + 1) >> 1) & 1) : wait(b_pv, 0);

@@ -35,7 +35,8 @@
 // 79 us (4.9 / 4.5 / 3.5 TB/s), D = 64 38 / 40 / 55 us. About 7 us are the line's start
 // and its join; at 32 heads HBM moves the rest at 5.6 TB/s, with a third of the issue
 // slots and of the tensor pipe busy. At W = 8 the chain of one step after another
-// (S, softmax, P) bounds it: the tensor memory has no room for a second block's.
+// (S, softmax, P) bounds it: tensor memory has no room for a second block's, or at
+// D = 64 where it has, 10 warps of 96 registers are no faster (58 us).
 #pragma once
 #include "fa_fwd.cuh"
 #include "fa_paged.cuh"

@@ -2,7 +2,10 @@
 against a request-by-request allocator in Python, the copies bit for bit, the
 attention against its formula in 64 bits."""
 import math
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -389,6 +392,29 @@ def test_attn_wide_pages(cuda, ps, layout):
         skip.add((r, j))
     check_attn(*s, *paged.paged_attn(*s), skip=skip)
     _lib.device_error(0)
+
+
+def test_attn_wide_checked_build(cuda):
+    """The wide groups' kernel in the checked library, whose TMA copies test their
+    coordinates and alignment first."""
+    import _build
+    _build.build(checked=True)
+    paths = [os.path.dirname(os.path.abspath(x)) for x in (__file__, paged.__file__)]
+    code = f"""
+import sys
+sys.path[:0] = {paths!r}
+import test_gpu_paged as t
+dev = t.torch.device("cuda", 0)
+t._lib.tma_check_word(0, reset=True)
+for D, heads in ((64, 40), (128, 40), (64, 100), (128, 100)):
+    s = t.scene(dev, 160, heads, 1, D, 48, [(7 * i) % 500 for i in range(160)], t.torch.bfloat16)
+    t.check_attn(*s, *t.paged.paged_attn(*s))
+print(t.os.path.basename(t._lib.loaded_path()), t._lib.tma_check_word(0), t._lib.device_error(0))
+"""
+    res = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, FA_B200_DEBUG="1"),
+                         capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stdout[-2000:] + res.stderr[-4000:]
+    assert res.stdout.split()[-3:] == ["libfa_b200_debug.so", "0", "0"]
 
 
 def test_attn_outputs(cuda):

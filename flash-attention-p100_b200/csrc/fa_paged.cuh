@@ -656,8 +656,8 @@ struct Line {
   int blocks;            // blocks that have a stretch
 };
 struct LineShared {
-  long long sums[8], first;  // first: the stretch's first step in its request
-  int b;                     // that request
+  long long sums[16], first;  // a sum per warp; first: the stretch's first step in its request
+  int b;                      // that request
 };
 
 // Adds up the lengths, divides the line, finds this block's stretch and deals
@@ -665,6 +665,7 @@ struct LineShared {
 template <int STEP, int D, int THREADS>
 __device__ __forceinline__ long long line_begin(const PagedAttnArgs& a, int units, bool by_unit, Line& line,
                                                 LineShared& shared) {
+  static_assert(THREADS / 32 <= static_cast<int>(sizeof(shared.sums) / sizeof(shared.sums[0])), "a sum per warp");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const auto steps = [&](int b) { return (request_len(a, b) + STEP - 1) / STEP; };
   const int per = (a.B + THREADS - 1) / THREADS;

@@ -405,7 +405,7 @@ int paged_attn_impl(PagedAttnArgs& a, const PagedPlan& p, const Strides& sk, con
   return launch_after(paged_join_kernel<D, BF>, "paged_join_kernel",
                       dim3(static_cast<unsigned>(std::min(p.units, p.blocks)),
                            (cols + most_cols - 1) / most_cols),
-                      kJoinThreads, 0, 0, stream, a, p.rows, most_cols);
+                      kJoinThreads, 0, 0, stream, a, p.rows, most_cols, static_cast<int>(p.blocks));
 }
 
 // An fp32 dQ is produced by the fused kernel: one pass, dQ added into the

@@ -1122,13 +1122,21 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
 // maximum; the threads of a column meet in shared memory.
 constexpr int kJoinThreads = 256;
 
+// Whether a record names a unit of the call and blocks of its launch. A block of
+// paged_wide_kernel that gave up a wait leaves without its records, and a workspace
+// does not start at zero: what is there instead must address nothing.
+__host__ __device__ constexpr bool record_in_range(int unit, int first, int last, long long units, long long blocks) {
+  return unit >= 0 && unit < units && first >= 0 && first <= last && last < blocks;
+}
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int row_tile, int most) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int row_tile, int most,
+                                                                   int blocks) {
   __shared__ float4 s_o[kJoinThreads];
   __shared__ float2 s_ml[kJoinThreads];
   wait_for_prior_launch();
   const int4 record = a.split[blockIdx.x];
-  if (record.x < 0) return;
+  if (!record_in_range(record.x, record.y, record.z, static_cast<long long>(a.B) * a.Hkv * a.row_tiles, blocks)) return;
   const int group = a.Hq / a.Hkv, rows = min(group, row_tile);
   const int rt = record.x % a.row_tiles, b = record.x / (a.row_tiles * a.Hkv);
   const int head0 = (record.x / a.row_tiles - b * a.Hkv) * group + rt * row_tile;

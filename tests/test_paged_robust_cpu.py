@@ -26,3 +26,20 @@ def test_the_line_has_a_sum_per_warp(tmp_path, warps):
 static_assert(sizeof(fab::LineShared::sums) / sizeof(long long) >= {warps}, "fewer sums than warps");
 """)
     assert ok, err
+
+
+def test_the_join_follows_no_record_that_was_not_written(tmp_path):
+    """A block that gave up a wait has written no record: whatever the workspace holds
+    there must name a unit of the call and blocks of its launch, or be passed over."""
+    int_max, int_min = 2 ** 31 - 1, -2 ** 31
+    units, blocks = 12, 7
+    good = [(0, 0, 0), (11, 0, 6), (5, 6, 6)]
+    bad = [(-1, 0, 0), (12, 0, 0), (int_max, 0, 0), (int_min, 0, 0), (3, -1, 2), (3, int_min, 2), (3, 5, 4),
+           (3, 0, 7), (3, 0, int_max), (3, int_max, int_min)]
+    checks = [f"static_assert({'' if r in good else '!'}fab::record_in_range({r[0]}ll, {r[1]}ll, {r[2]}ll, "
+              f"{units}, {blocks}));" for r in good + bad]
+    ok, err = compiles(tmp_path, "#include <cuda.h>\n#include \"fa_paged.cuh\"\n" + "\n".join(checks))
+    assert ok, err
+    # the kernel asks before it uses one
+    body = open(os.path.join(_build.CSRC, "fa_paged.cuh")).read().split("paged_join_kernel(const", 1)[1]
+    assert body.index("record_in_range(record.x, record.y, record.z") < body.index("record.x %")

@@ -562,10 +562,12 @@ struct PartSum {
 template <bool BF>
 __device__ __forceinline__ constexpr float weight_bias() { return BF ? 0.f : 7.f; }
 
-// Writes columns col .. col + 3 of a head's result.
+// Writes columns col .. col + 3 of a head's result. Weights that sum to 0 (no key with
+// a page, or every score -inf) give what a request without a token gets, o = 0 beside
+// lse = -inf, and not 0 / 0.
 template <bool BF>
 __device__ __forceinline__ void store_part_sum(const PagedAttnArgs& a, const PartSum& x, int b, int head, int col) {
-  const float inv = 1.f / x.l;
+  const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
   *reinterpret_cast<uint2*>(a.o + a.so.at(b, head, 0) + col) =
       make_uint2(pack16<BF>(x.o.x * inv, x.o.y * inv), pack16<BF>(x.o.z * inv, x.o.w * inv));
   if (col == 0)

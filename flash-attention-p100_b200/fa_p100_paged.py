@@ -99,8 +99,10 @@ def paged_attn(q, k_cache, v_cache, block_table, lens):
     cached tokens 0 .. lens[r] - 1 (the new token among them once it is appended).
     Returns (o, lse): o (B, Hq, D) in q's dtype, lse (B, Hq) fp32, natural log, as
     `fa_p100_ext.forward` gives them, in one allocation; a request of length 0 gets
-    o = 0 and lse = -inf. Hq is a multiple of Hkv; what lies behind a request's last token in its
-    last page is never used, whatever it holds. The same inputs give the same bits."""
+    o = 0 and lse = -inf, and so does a head with nothing to add up: every token's
+    page outside the cache, or every score -inf. Hq is a multiple of Hkv; what lies behind
+    a request's last token in its last page is never used, whatever it holds. The same
+    inputs give the same bits."""
     return _native.attn(q, k_cache, v_cache, block_table, lens)
 
 

@@ -204,8 +204,10 @@ size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, 
  * (fa_b200_strides batch and head; row is not used). A length below 0 counts as
  * 0, one above W * page_size as W * page_size; a row of length 0 gets o = 0 and
  * lse = -inf. What lies behind a request's last token is never used. A table
- * entry outside [0, P) sets FA_B200_DEVERR_PAGE and its tokens are left out. The
- * result does not depend on timing: equal inputs give equal bits. */
+ * entry outside [0, P) sets FA_B200_DEVERR_PAGE and its tokens are left out. A head
+ * whose weights sum to 0, as every token is left out or every score is -inf, gets
+ * o = 0 and lse = -inf too. The result does not depend on timing: equal inputs give
+ * equal bits. */
 int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, fa_b200_strides skc,
                        const void* v_cache, fa_b200_strides svc, const int* block_table,
                        int64_t table_stride, const int* lens, void* o, fa_b200_strides so,

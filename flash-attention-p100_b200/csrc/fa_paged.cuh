@@ -432,8 +432,8 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // line is paged_wide_kernel's: two fragments' products at 8 warps an SM are bound by
 // their latency, 85 us at 32 heads. Clusters take them here, up to 32 heads a tile.
 
-// Strides of a cache in units of 16 bytes (page, head, token): products of 32
-// bits, one instruction each, that still span 64 GB.
+// Strides of a cache in units of 16 bytes (page, head, token): 32 bits each, so a
+// stride may be 64 GB, and one instruction for each product, which has 64.
 struct Units {
   uint32_t b, h, n;
 };
@@ -852,16 +852,16 @@ __global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnArgs a) 
 #pragma unroll
         for (int i = 0; i < 16 / RPI; ++i) {
           const uint32_t to = (d ^ (((i * RPI) & 7) << 4)) + i * RPI * (D * 2);
-          cp_async16(to, k + i * RPI * a.skc.n);
-          cp_async16(to + C::TILE, v + i * RPI * a.svc.n);
+          cp_async16(to, unit_at(k, a.skc, 0, 0, i * RPI));
+          cp_async16(to + C::TILE, unit_at(v, a.svc, 0, 0, i * RPI));
         }
       } else if (left > 0) {   // rows behind the last token are filled with zeros, not read
 #pragma unroll
         for (int i = 0; i < 16 / RPI; ++i) {
           const uint32_t to = (d ^ (((i * RPI) & 7) << 4)) + i * RPI * (D * 2);
           const int bytes = i * RPI + lr < n ? 16 : 0;
-          cp_async16(to, k + i * RPI * a.skc.n, bytes);
-          cp_async16(to + C::TILE, v + i * RPI * a.svc.n, bytes);
+          cp_async16(to, unit_at(k, a.skc, 0, 0, i * RPI), bytes);
+          cp_async16(to + C::TILE, unit_at(v, a.svc, 0, 0, i * RPI), bytes);
         }
       }
     }

@@ -67,3 +67,34 @@ def test_attn_with_nothing_left(cuda, case, D, dtype):
     o, lse = paged.paged_attn(q2, k2, vc, table, lens)
     assert (o[0, -1] == 0).all() and (lse[0, -1] == -float("inf")).all()
     assert torch.equal(bits(o[1:]), bits(clean[0][1:])) and torch.equal(lse[1:], clean[1][1:])
+
+
+@pytest.mark.parametrize("D,units", [(64, 357913942), (128, 306783379)])
+@pytest.mark.parametrize("heads", [(8, 2), (40, 2)], ids=["8", "40"])
+def test_attn_token_strides_past_32_bits(cuda, D, units, heads):
+    """Pages stored token by token over the whole pool, so that the tokens of a page lie
+    4.9 GB apart (D = 128) or 5.7 GB: 14 (12) rows times the stride in units of 16 bytes
+    is 2^32 and a little. Only the rows of this test's pages are ever touched."""
+    Hkv, ps, P, n = 2, 16, 40, units * 8
+    need = (ps - 1) * n + 2 * P * Hkv * D
+    torch.cuda.empty_cache()
+    assert torch.cuda.mem_get_info(cuda)[0] > 2 * need
+    flat = torch.empty(need, dtype=torch.float16, device=cuda)
+    kc, vc = (flat.as_strided((P, Hkv, ps, D), (2 * Hkv * D, D, n, 1), at * Hkv * D) for at in (0, 1))
+    gen = torch.Generator(device=cuda).manual_seed(D)
+    for t in range(ps):
+        for c in (kc, vc):
+            c[:, :, t] = torch.randn(P, Hkv, D, device=cuda, generator=gen).half()
+    # clusters, and more units than they take
+    for lens in ([500, 37], [1 + 7 * i % 300 for i in range(200)]):
+        pages = torch.arange(len(lens) * 38, device=cuda).view(len(lens), 38) * 7 % P
+        q = torch.randn(len(lens), heads[0], D, device=cuda, generator=gen).half()
+        s = (q, kc, vc, pages.to(torch.int32), torch.tensor(lens, dtype=torch.int32, device=cuda))
+        check_attn(*s, *paged.paged_attn(*s))
+    rows = torch.randn(3, Hkv, D, device=cuda, generator=gen).half()
+    paged.paged_append(rows, -rows, torch.tensor([15, 3 * 16 + 14, P * 16 - 1], dtype=torch.int32, device=cuda), kc, vc)
+    for i, (page, t) in enumerate(((0, 15), (3, 14), (P - 1, 15))):
+        assert torch.equal(kc[page, :, t], rows[i]) and torch.equal(vc[page, :, t], -rows[i])
+    fa_p100.check_device_errors(cuda)
+    del flat, kc, vc, s
+    torch.cuda.empty_cache()

@@ -169,6 +169,13 @@ void no_grad(std::initializer_list<Named> all) {
       refuse("the paged cache has no backward: call it under torch.no_grad() or detach ", x.name);
 }
 
+// A caller's tensor that a call has written changes as under torch's own in-place
+// operations: a backward that saved it (or a view) raises. Inference tensors have no
+// version.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // On the device of the call from here on; outputs are plain allocations there.
 struct Call {
   c10::cuda::CUDAGuard device;
@@ -225,9 +232,12 @@ struct TableOutputs {
   static constexpr int64_t kFewSlots = 16384;
   at::Tensor all, granted, slots, lens, free_count;
   size_t ws_bytes;
+  bool own_lens, own_free_count;   // no caller's
   TableOutputs(const Requests& r, bool extends, int64_t total, pybind11::handle lens_out,
                pybind11::handle free_count_out)
-      : ws_bytes(abi.table_workspace_bytes(static_cast<int>(r.B))) {
+      : ws_bytes(abi.table_workspace_bytes(static_cast<int>(r.B))),
+        own_lens(lens_out.is_none()),
+        own_free_count(free_count_out.is_none()) {
     const int64_t few = total <= kFewSlots ? total : 0, more = extends ? r.B + few : 0;
     const int64_t ws = (static_cast<int64_t>(ws_bytes) + 3) / 4 * 4;
     all = bytes_of(ws + 4 * (more + r.B + 1), r.lens);
@@ -236,8 +246,12 @@ struct TableOutputs {
       granted = ints_at(0, r.B);
       slots = few == total ? ints_at(r.B, total) : empty({total}, r.lens, at::kInt);
     }
-    lens = lens_out.is_none() ? ints_at(more, r.B) : given(lens_out, "lens_out", r.lens);
-    free_count = free_count_out.is_none() ? ints_at(more + r.B, 1) : given(free_count_out, "free_count_out", r.free_count);
+    lens = own_lens ? ints_at(more, r.B) : given(lens_out, "lens_out", r.lens);
+    free_count = own_free_count ? ints_at(more + r.B, 1) : given(free_count_out, "free_count_out", r.free_count);
+  }
+  void mark_written() const {
+    if (!own_lens) written(lens);
+    if (!own_free_count) written(free_count);
   }
   static at::Tensor given(pybind11::handle h, const char* name, const at::Tensor& like) {
     const at::Tensor& t = ints(h, name, like.numel());
@@ -261,6 +275,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> extend(
                           out.all.data_ptr(), out.ws_bytes, static_cast<int>(r.B), static_cast<int>(r.table.W), static_cast<int>(r.P),
                           static_cast<int>(page), static_cast<int>(total), call.stream),
                "fa_b200_paged_extend");
+  written(r.table.t);
+  out.mark_written();
   return {out.slots, out.granted, out.lens, out.free_count};
 }
 
@@ -278,6 +294,8 @@ std::tuple<at::Tensor, at::Tensor> release(pybind11::handle finished, pybind11::
                            data(out.free_count), out.all.data_ptr(), out.ws_bytes, static_cast<int>(r.B), static_cast<int>(r.table.W), static_cast<int>(r.P),
                            static_cast<int>(page), call.stream),
                "fa_b200_paged_release");
+  written(r.free_pages);
+  out.mark_written();
   return {out.lens, out.free_count};
 }
 
@@ -310,6 +328,8 @@ void append(pybind11::handle k_new, pybind11::handle v_new, pybind11::handle slo
                           static_cast<int>(T), static_cast<int>(c.Hkv), static_cast<int>(c.D),
                           static_cast<int>(c.P), static_cast<int>(c.page), c.dtype, call.stream),
                "fa_b200_paged_append");
+  written(c.k);
+  written(c.v);
 }
 
 std::tuple<at::Tensor, at::Tensor> attn(pybind11::handle query, pybind11::handle k_cache, pybind11::handle v_cache,

@@ -98,3 +98,44 @@ def test_attn_token_strides_past_32_bits(cuda, D, units, heads):
     fa_p100.check_device_errors(cuda)
     del flat, kc, vc, s
     torch.cuda.empty_cache()
+
+
+def i32(values, dev):
+    return torch.tensor(values, dtype=torch.int32, device=dev)
+
+
+def test_writes_are_seen_by_autograd(cuda):
+    """What the operators write counts as changed in place: a backward that saved it
+    raises, as after torch's own in-place operations."""
+    c = paged.PagedKVCache(2, 2, 64, 9, 3, 48, 16, torch.float16, cuda)
+    rows = torch.ones(3, 2, 64, device=cuda).half()
+    tensors = dict(k=c.k, v=c.v, table=c.block_table, lens=c.lens, free=c.free_pages, count=c.free_count)
+
+    def changed(call):
+        before = {n: t._version for n, t in tensors.items()}
+        call()
+        return {n for n, t in tensors.items() if t._version != before[n]}
+
+    w = torch.ones(64, device=cuda).half().requires_grad_(True)
+    for saved in (c.k, c.k[1], c.v[1, 0]):
+        c.extend(i32([1, 1, 1], cuda), 3)
+        y = (saved * w).sum()      # saves the cache, or a view of it, for w's gradient
+        with torch.no_grad():
+            c.append(1, rows, rows)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    assert changed(lambda: c.extend(i32([1, 1, 1], cuda), 3)) == {"table", "lens", "count"}
+    assert changed(lambda: c.append(0, rows, rows)) == {"k", "v"}
+    assert changed(lambda: c.attn(0, rows)) == set()
+    assert changed(lambda: c.release(torch.tensor([True, False, True], device=cuda))) == {"free", "lens", "count"}
+    # outputs of the call's own leave the inputs as they were
+    assert changed(lambda: paged.paged_extend(i32([1, 0, 0], cuda), c.lens, c.block_table, c.free_pages, c.free_count,
+                                              16, 1)) == {"table"}
+    # inference tensors have no version; outside inference mode they are written all the same
+    with torch.inference_mode():
+        c = paged.PagedKVCache(1, 2, 64, 9, 3, 48, 16, torch.float16, cuda)
+        c.extend(i32([1, 1, 1], cuda), 3)
+        c.append(0, rows, rows)
+    c.extend(i32([1, 0, 0], cuda), 1)
+    c.append(0, rows[:1], rows[:1])
+    assert c.lens.tolist() == [2, 1, 1] and float(c.k.float().sum()) == 4 * 2 * 64

@@ -162,11 +162,16 @@ at::Device one_device(std::initializer_list<Named> all) {
   return device;
 }
 
+// Forward-mode tangents are refused under torch.no_grad() too, which does not turn
+// that mode off.
 void no_grad(std::initializer_list<Named> all) {
-  if (!c10::GradMode::is_enabled()) return;
-  for (const Named& x : all)
-    if (x.t.requires_grad())
+  const bool records = c10::GradMode::is_enabled();
+  for (const Named& x : all) {
+    if (records && x.t.requires_grad())
       refuse("the paged cache has no backward: call it under torch.no_grad() or detach ", x.name);
+    if (x.t._fw_grad(0).defined())
+      refuse("the paged cache has no forward-mode derivative: ", x.name, " carries a tangent");
+  }
 }
 
 // A caller's tensor that a call has written changes as under torch's own in-place

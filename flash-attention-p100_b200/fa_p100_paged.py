@@ -28,7 +28,9 @@ be served is refused (granted 0, slots -1), and a table entry that names no page
 of the cache leaves its tokens out of the attention and sets the device error
 word, which `fa_p100.check_device_errors()` reports. Arguments the host can check raise
 RuntimeError before anything is launched. There is no backward: tensors that
-require a gradient are refused while gradients are recorded.
+require a gradient are refused while gradients are recorded, and ones that carry a
+forward-mode tangent always. What an operator writes in place counts as changed for
+a backward that saved it.
 """
 import ctypes
 

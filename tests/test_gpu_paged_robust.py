@@ -139,3 +139,31 @@ def test_writes_are_seen_by_autograd(cuda):
     c.extend(i32([1, 0, 0], cuda), 1)
     c.append(0, rows[:1], rows[:1])
     assert c.lens.tolist() == [2, 1, 1] and float(c.k.float().sum()) == 4 * 2 * 64
+
+
+def test_transforms_and_fake_tensors_are_refused(cuda):
+    """torch.func's wrappers, dual and fake tensors: refused, nothing written."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    import torch.autograd.forward_ad as fwAD
+    half = lambda *s: torch.randn(*s, device=cuda).half()
+    a = dict(k=half(5, 2, 64), v=half(5, 2, 64), slots=i32([0, 1, 2, 3, 20], cuda), k_cache=half(4, 2, 16, 64),
+             v_cache=half(4, 2, 16, 64))
+    b = dict(q=half(3, 4, 64), k_cache=a["k_cache"], v_cache=a["v_cache"], block_table=i32([[0, 1]] * 3, cuda),
+             lens=i32([1, 20, 3], cuda))
+    kept = a["k_cache"].clone(), a["v_cache"].clone()
+    for op, args in ((paged.paged_append, a), (paged.paged_attn, b)):
+        for name, x in args.items():
+            def call(t):
+                op(**{**args, name: t})
+                return t
+            with pytest.raises(RuntimeError):
+                torch.func.vmap(call)(x[None])
+            if x.is_floating_point():
+                with pytest.raises(RuntimeError):
+                    torch.func.jvp(call, (x,), (torch.ones_like(x),))
+                with fwAD.dual_level(), pytest.raises(RuntimeError, match="carries a tangent"):
+                    call(fwAD.make_dual(x, torch.ones_like(x)))
+        with FakeTensorMode(allow_non_fake_inputs=True) as mode, pytest.raises(RuntimeError):
+            op(**{n: mode.from_tensor(t) for n, t in args.items()})
+    torch.cuda.synchronize()
+    assert torch.equal(a["k_cache"], kept[0]) and torch.equal(a["v_cache"], kept[1])

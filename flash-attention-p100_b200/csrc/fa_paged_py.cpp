@@ -147,6 +147,61 @@ Caches caches(pybind11::handle hk, pybind11::handle hv) {
   return c;
 }
 
+// Whether two tensors share a byte. Their elements are sums of index times stride, so
+// they do if some difference of indices makes up the distance of their bases: looked
+// for axis by axis, the largest stride first, with what the smaller ones can still make
+// up as the bound. Caches, rows and slices of one buffer have strides that nest, and
+// leave at most two choices an axis. Layouts that leave many more count as shared.
+struct Axis {
+  int64_t stride, lo, hi;   // bytes; differences of indices
+};
+bool makes_up(const Axis* axis, const Axis* end, int64_t distance, int& budget) {
+  if (axis == end) return distance == 0;
+  int64_t lo = 0, hi = 0;   // of the smaller strides
+  for (const Axis* x = axis + 1; x != end; ++x) {
+    lo += x->lo * x->stride;
+    hi += x->hi * x->stride;
+  }
+  const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  const int64_t first = std::max(axis->lo, -floor_div(hi - distance, axis->stride));
+  const int64_t last = std::min(axis->hi, floor_div(distance - lo, axis->stride));
+  for (int64_t i = first; i <= last; ++i)
+    if (--budget < 0 || makes_up(axis + 1, end, distance - i * axis->stride, budget)) return true;
+  return false;
+}
+bool share_memory(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto bytes = [](const at::Tensor& t) {   // from the first element to behind the last
+    int64_t n = t.element_size();
+    for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i) * t.element_size();
+    return n;
+  };
+  const int64_t distance =
+      static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()) - reinterpret_cast<uintptr_t>(a.data_ptr()));
+  if (distance >= bytes(a) || -distance >= bytes(b)) return false;
+  Axis axes[16];   // the tensors have up to 4 axes each
+  int n = 0;
+  const auto add = [&](int64_t stride, int64_t lo, int64_t hi) {
+    if (stride == 0 || lo == hi) return;
+    int i = 0;
+    while (i < n && axes[i].stride > stride) ++i;
+    if (i < n && axes[i].stride == stride) {
+      axes[i].lo += lo;
+      axes[i].hi += hi;
+      return;
+    }
+    std::copy_backward(axes + i, axes + n, axes + n + 1);
+    axes[i] = {stride, lo, hi};
+    ++n;
+  };
+  for (int64_t i = 0; i < a.dim(); ++i) add(a.stride(i) * a.element_size(), 0, a.size(i) - 1);
+  for (int64_t i = 0; i < b.dim(); ++i) add(b.stride(i) * b.element_size(), 1 - b.size(i), 0);
+  add(1, 0, a.element_size() - 1);   // an element's bytes
+  add(1, 1 - b.element_size(), 0);
+  int budget = 10000;
+  return makes_up(axes, axes + n, distance, budget);
+}
+
 struct Named {
   const char* name;
   const at::Tensor& t;
@@ -321,7 +376,9 @@ void append(pybind11::handle k_new, pybind11::handle v_new, pybind11::handle slo
   for (const fa_b200_strides& st : {c.sk, c.sv})
     if (st.batch == 0 || st.head == 0 || st.row == 0)
       refuse("k_cache and v_cache are written and must not be expanded views");
-  if (c.k.data_ptr() == c.v.data_ptr()) refuse("k_cache and v_cache must be different memory");
+  if (share_memory(c.k, c.v)) refuse("k_cache and v_cache must be different memory");
+  for (const Named& x : {Named{"k", k}, Named{"v", v}, Named{"slots", s}})
+    if (share_memory(x.t, c.k) || share_memory(x.t, c.v)) refuse(x.name, " must not overlap the caches");
   no_grad({{"k", k}, {"v", v}, {"k_cache", c.k}, {"v_cache", c.v}});
   Call call(one_device({{"k_cache", c.k}, {"v_cache", c.v}, {"k", k}, {"v", v}, {"slots", s}}));
   if (T == 0) return;

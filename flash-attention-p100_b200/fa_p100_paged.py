@@ -91,8 +91,9 @@ def paged_append(k, v, slots, k_cache, v_cache):
     """Writes the keys and values (T, Hkv, D) of T tokens into their slots of the
     caches, in place. slots is int32 (T,); a token whose slot is outside the cache
     (-1) is skipped, the others' slots must differ from each other. k and v may be
-    strided views (slices of a fused projection) outside the caches; they have the
-    caches' dtype."""
+    strided views (slices of a fused projection); they have the caches' dtype. Caches
+    that share memory with each other, k, v or slots are refused; slices of one
+    buffer that interleave without an element in common are not."""
     _native.append(k, v, slots, k_cache, v_cache)
 
 

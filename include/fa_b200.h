@@ -187,7 +187,8 @@ int fa_b200_paged_release(const unsigned char* finished, const int* lens, const 
 /* Writes T tokens' keys and values into their slots: k_cache[slot] = k[t],
  * v_cache[slot] = v[t]. k and v are (T, Hkv, D) with D contiguous
  * (fa_b200_strides head and row; batch is not used). Tokens whose slot is not in
- * [0, P * page_size) are skipped; the others' slots must differ from each other. */
+ * [0, P * page_size) are skipped; the others' slots must differ from each other.
+ * k_cache and v_cache must not overlap each other, k, v or slots (not checked). */
 int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b200_strides sv,
                          const int* slots, void* k_cache, fa_b200_strides skc, void* v_cache,
                          fa_b200_strides svc, int T, int Hkv, int D, int P, int page_size,

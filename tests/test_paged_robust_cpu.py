@@ -1,5 +1,6 @@
 """The paged cache's sizes and refusals that need no GPU, beside test_paged_cpu.py."""
 import os
+import random
 import subprocess
 
 import pytest
@@ -96,3 +97,91 @@ def test_transformed_and_fake_tensors_are_refused(op, args, name):
         b = {n: mode.from_tensor(t) for n, t in a.items()}
         with pytest.raises(RuntimeError):
             op(**b)
+
+
+def slices(name):
+    """Two caches of (4, 2, 16, 64) out of one buffer, and whether they share memory."""
+    shape = (4, 2, 16, 64)
+    b = torch.zeros(1 << 16, dtype=torch.float16)
+    page = 2 * 16 * 64
+    view = lambda at, *stride: b.as_strided(shape, stride, at)
+    head = (page, 1024, 64, 1)
+    return {
+        "next to each other": ((view(0, *head), view(4 * page, *head)), False),
+        "last page and first": ((view(0, *head), view(3 * page, *head)), True),
+        "heads 0-1 and 1-2 of 3": ((view(0, 3072, 1024, 64, 1), view(1024, 3072, 1024, 64, 1)), True),
+        "heads 0-1 and 2-3 of 4": ((view(0, 4096, 1024, 64, 1), view(2048, 4096, 1024, 64, 1)), False),
+        "pages in turn": ((view(0, 2 * page, 1024, 64, 1), view(page, 2 * page, 1024, 64, 1)), False),
+        "pages in turn, a row over": ((view(0, 2 * page, 1024, 64, 1), view(page - 64, 2 * page, 1024, 64, 1)), True),
+        "by token, k and v in turn": ((view(0, 16 * 256, 64, 256, 1), view(128, 16 * 256, 64, 256, 1)), False),
+        "by token, one head over": ((view(0, 16 * 192, 64, 192, 1), view(64, 16 * 192, 64, 192, 1)), True),
+        "rows in turn": ((view(0, 2 * page, 2048, 128, 1), view(64, 2 * page, 2048, 128, 1)), False),
+        "half a row": ((view(0, 2 * page, 2048, 128, 1), view(32, 2 * page, 2048, 128, 1)), True),
+        "page's first 8 bytes": ((view(0, *head), view(4 * page - 8, *head)), True),
+        "two layouts apart": ((view(0, *head), view(4 * page, page, 64, 128, 1)), False),
+        "two layouts over": ((view(0, *head), view(3 * page + 1024, page, 64, 128, 1)), True),
+        "two layouts in turn": ((view(0, 2 * page, 1024, 64, 1), view(page, 2 * page, 64, 128, 1)), False),
+    }[name]
+
+
+@pytest.mark.parametrize("name", [
+    "next to each other", "last page and first", "heads 0-1 and 1-2 of 3", "heads 0-1 and 2-3 of 4", "pages in turn",
+    "pages in turn, a row over", "by token, k and v in turn", "by token, one head over", "rows in turn", "half a row",
+    "page's first 8 bytes", "two layouts apart", "two layouts over", "two layouts in turn"])
+def test_append_refuses_caches_that_share_memory(name):
+    (k, v), shared = slices(name)
+    # what the views really touch
+    marks = torch.zeros(1 << 16, dtype=torch.int32)
+    for x in (k, v):
+        marks.as_strided(x.shape, x.stride(), x.storage_offset()).add_(1)
+    assert bool((marks > 1).any()) == shared
+    for a, b in ((k, v), (v, k)):
+        with pytest.raises(RuntimeError, match="different memory" if shared else "CUDA"):
+            paged.paged_append(**{**append_args(), "k_cache": a, "v_cache": b})
+
+
+@pytest.mark.parametrize("name", ["k", "v", "slots"])
+@pytest.mark.parametrize("cache", [0, 1])
+def test_append_refuses_rows_inside_the_caches(name, cache):
+    """k, v and slots in a cache's memory, in the gap between its pages, and behind it."""
+    page = 2 * 16 * 64
+    b = torch.zeros(10 * page, dtype=torch.float16)
+    gaps = b.as_strided((4, 2, 16, 64), (2 * page, 1024, 64, 1))      # every other page
+    for at, shared in ((0, True), (7 * page, False), (6 * page + 1024, True), (page, False), (page - 8, True),
+                       (page + 1024, False), (2 * page - 8, True), (8 * page, False)):
+        if name == "slots":
+            x = b.view(torch.int32)[at // 2:][:5]
+        else:
+            x = b[at:][:5 * 128].view(5, 2, 64)
+        a = append_args()
+        a[name], a[("k_cache", "v_cache")[cache]] = x, gaps
+        with pytest.raises(RuntimeError, match=f"{name} must not overlap" if shared else "CUDA"):
+            paged.paged_append(**a)
+
+
+def test_append_overlap_against_every_element():
+    """Random layouts of one buffer: refused exactly where an element is in both."""
+    rng = random.Random(0)
+    n = 0
+    for _ in range(300):
+        def layout():
+            axes = [(4, None), (2, None), (16, None)]
+            order = rng.sample(range(3), 3)
+            stride, at = [0, 0, 0], 64 + 8 * rng.randrange(3)
+            for i in order:
+                stride[i] = at * rng.choice([1, 1, 2])
+                at = stride[i] * axes[i][0] + 8 * rng.randrange(2)
+            return (*stride, 1)
+        sk = layout()
+        sv = sk if rng.random() < 0.7 else layout()
+        off = rng.choice([64, 72, 1024, 2048, sk[0], sk[1], sk[2], sk[1] // 2 // 8 * 8, 4 * sk[0], 8 * rng.randrange(900)])
+        b = torch.zeros(off + 4 * max(sk[0], sk[1], sk[2], sv[0], sv[1], sv[2]) * 16, dtype=torch.float16)
+        k, v = (b.as_strided((4, 2, 16, 64), s, o) for s, o in ((sk, 0), (sv, off)))
+        marks = torch.zeros(b.numel(), dtype=torch.bool)
+        marks.as_strided(k.shape, k.stride(), 0).fill_(True)
+        shared = bool(marks.as_strided(v.shape, v.stride(), off).any())
+        with pytest.raises(RuntimeError) as e:
+            paged.paged_append(**{**append_args(), "k_cache": k, "v_cache": v})
+        assert ("different memory" in str(e.value)) == shared, (sk, sv, off)
+        n += shared
+    assert 0 < n < 300     # both kinds were among them

@@ -6,6 +6,7 @@ C-ABI shared object compiled by nvcc for sm_100a only, built in-tree so it
 travels with the source tree; `build()` is idempotent and skips the compile
 when the library is newer than every source file.
 """
+import hashlib
 import os
 import shutil
 import subprocess
@@ -91,12 +92,32 @@ BINDING_SOURCE = os.path.join(CSRC, "fa_paged_py.cpp")
 BINDING_PATH = os.path.join(HERE, "_fa_paged.so")
 
 
+def _binding_flags():
+    import torch
+    return ["-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+
+
+def binding_key():
+    """What the module is compiled against: it uses torch's and Python's class layouts,
+    so it serves the torch, the interpreter and the flags it was built with alone."""
+    import sysconfig
+
+    import torch
+    parts = [torch.__version__, str(torch.version.git_version), str(sysconfig.get_config_var("EXT_SUFFIX")),
+             *_binding_flags()]
+    return "fa_paged-" + hashlib.sha256("\0".join(parts).encode()).hexdigest()
+
+
 def binding_up_to_date():
+    """Newer than its sources, and of this binding_key(), which the module holds: read
+    from the file, as a module of another torch must not be loaded to ask it."""
     if not os.path.exists(BINDING_PATH):
         return False
     built = os.path.getmtime(BINDING_PATH)
-    return all(os.path.getmtime(s) <= built
-               for s in (BINDING_SOURCE, os.path.join(INCLUDE, "fa_b200.h")))
+    if any(os.path.getmtime(s) > built for s in (BINDING_SOURCE, os.path.join(INCLUDE, "fa_b200.h"))):
+        return False
+    with open(BINDING_PATH, "rb") as f:
+        return binding_key().encode() in f.read()
 
 
 def build_binding(force=False):
@@ -110,8 +131,8 @@ def build_binding(force=False):
     home = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc()))
     tmp = f"{BINDING_PATH}.{os.getpid()}.tmp"
-    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", *_binding_flags(),
+           f'-DFA_PAGED_KEY="{binding_key()}"',
            f"-I{home}/include", f"-I{home}/include/torch/csrc/api/include",
            f"-I{sysconfig.get_path('include')}", f"-I{cuda}/include", BINDING_SOURCE, "-o", tmp,
            f"-L{home}/lib", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]

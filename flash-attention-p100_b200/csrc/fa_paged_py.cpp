@@ -431,6 +431,7 @@ std::tuple<at::Tensor, at::Tensor> attn(pybind11::handle query, pybind11::handle
 }  // namespace
 
 PYBIND11_MODULE(_fa_paged, m) {
+  m.attr("build_key") = FA_PAGED_KEY;   // what this was compiled against (_build.binding_key)
   m.def("bind", &bind);
   m.def("extend", &extend);
   m.def("release", &release);

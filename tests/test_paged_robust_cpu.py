@@ -185,3 +185,32 @@ def test_append_overlap_against_every_element():
         assert ("different memory" in str(e.value)) == shared, (sk, sv, off)
         n += shared
     assert 0 < n < 300     # both kinds were among them
+
+
+def test_the_native_module_is_kept_for_its_torch_alone(monkeypatch, tmp_path):
+    """_fa_paged.so uses torch's class layouts: another torch, interpreter or flags mean
+    another module."""
+    import sysconfig
+    import _fa_paged
+    _build.build_binding()
+    assert _build.binding_up_to_date() and _fa_paged.build_key == _build.binding_key()
+    for target, name, value in ((torch, "__version__", "2.12.0"), (torch.version, "git_version", "0" * 40),
+                                (sysconfig, "get_config_var", lambda n: ".cpython-313-x86_64-linux-gnu.so"),
+                                (torch, "compiled_with_cxx11_abi", lambda: not ABI)):
+        with monkeypatch.context() as m:
+            m.setattr(target, name, value)
+            assert not _build.binding_up_to_date(), name
+    with monkeypatch.context() as m:     # asking needs no compiler
+        m.setattr(_build, "_nvcc", lambda: 1 / 0)
+        m.setenv("CXX", "/nowhere/c++")
+        assert _build.build_binding() == _build.BINDING_PATH
+    # a file cut short, newer than every source
+    cut = tmp_path / "_fa_paged.so"
+    cut.write_bytes(b"\x7fELF")
+    with monkeypatch.context() as m:
+        m.setattr(_build, "BINDING_PATH", str(cut))
+        assert not _build.binding_up_to_date()
+    assert _build.binding_up_to_date()
+
+
+ABI = torch.compiled_with_cxx11_abi()

@@ -39,6 +39,10 @@ class _PagedLayer(CacheLayerMixin):
     def update(self, key_states, value_states, *args, **kwargs):
         c = self._cache
         B, heads, N, D = key_states.shape
+        if self._tokens and N > 1:              # before anything is stored
+            raise NotImplementedError(
+                f"fa_p100 adds one token at a time to a cache that holds tokens ({self._tokens} here, "
+                f"{N} new); reset the cache, or run the prompt in one call")
         if B != c.batch:
             raise RuntimeError(f"this cache was made for a batch of {c.batch}, got {B}")
         if self._tokens == c.tokens:            # the first layer of a step

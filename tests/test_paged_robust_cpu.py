@@ -214,3 +214,46 @@ def test_the_native_module_is_kept_for_its_torch_alone(monkeypatch, tmp_path):
 
 
 ABI = torch.compiled_with_cxx11_abi()
+
+
+# ---- the HuggingFace cache, its operators recorded and not run ----
+def hf_model(layers=2, impl="fa_p100"):
+    import fa_p100_hf
+    from transformers import Qwen3Config, Qwen3ForCausalLM
+    cfg = Qwen3Config(vocab_size=64, hidden_size=128, intermediate_size=256, num_hidden_layers=layers,
+                      num_attention_heads=2, num_key_value_heads=1, head_dim=64, max_position_embeddings=64,
+                      tie_word_embeddings=True, attn_implementation="sdpa")
+    torch.manual_seed(0)
+    m = Qwen3ForCausalLM(cfg).eval()
+    return fa_p100_hf.enable_fa_p100(m) if impl == "fa_p100" else m
+
+
+def hf_cache(model, monkeypatch, batch=1, max_len=48):
+    """A cache whose calls of the GPU operators are listed, with attention in torch's own."""
+    import fa_p100_hf
+    cache, calls = fa_p100_hf.make_cache(model, batch, max_len), []
+    for name in ("extend", "append", "release", "attn"):
+        monkeypatch.setattr(cache.paged, name, lambda *a, name=name: (calls.append(name), a[-1])[1])
+    monkeypatch.setattr(fa_p100_hf, "_warned_cast", True)     # other tests look for the one warning
+    monkeypatch.setattr(fa_p100_hf, "flash_attn_bnhd", lambda q, k, v, causal, full_precision:
+                        torch.nn.functional.scaled_dot_product_attention(
+                            q, k, v, is_causal=causal, enable_gqa=True).transpose(1, 2))
+    return cache, calls
+
+
+def ids(n):
+    return torch.arange(n)[None]
+
+
+def test_hf_cache_refuses_a_second_prompt_unchanged(monkeypatch):
+    """The refusal comes before the prompt's keys are stored: the cache goes on as it was."""
+    model = hf_model()
+    cache, calls = hf_cache(model, monkeypatch)
+    with torch.no_grad():
+        model(ids(5), past_key_values=cache, use_cache=True)
+        assert calls == ["extend", "append", "append"] and cache.get_seq_length() == 5
+        with pytest.raises(NotImplementedError, match="one token at a time"):
+            model(ids(3), past_key_values=cache, use_cache=True)
+        assert calls == ["extend", "append", "append"] and cache.tokens == 5 and cache.get_seq_length() == 5
+        model(ids(1), past_key_values=cache, use_cache=True)
+    assert calls[3:] == ["extend", "append", "attn", "append", "attn"] and cache.get_seq_length() == 6

@@ -73,6 +73,8 @@ def fa_p100_attention_forward(module, query, key, value, attention_mask, dropout
     global _warned_cast
     # the paged cache marks the keys it has just stored
     layer, past = getattr(key, "_fa_p100_paged", (None, None))
+    if layer is not None:
+        layer.reached()
     reason = _unsupported(attention_mask, dropout, scaling, query, key, kwargs, past)
     if reason is not None:
         raise NotImplementedError(reason)

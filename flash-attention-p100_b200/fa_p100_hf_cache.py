@@ -13,8 +13,9 @@ fa_p100_paged.paged_attn over them. All sequences of a batch have one length, as
 the backend takes no padding. What it cannot do raises: a second prompt on a
 cache that already holds tokens (NotImplementedError), beam search and other
 calls that reorder or cut a cache (NotImplementedError), more than max_len tokens
-(RuntimeError), and, as the cache has no backward, keys that need a gradient
-(RuntimeError).
+(RuntimeError), a model whose attention is not "fa_p100" (RuntimeError: it would
+see the newest tokens alone), and, as the cache has no backward, keys that need a
+gradient (RuntimeError).
 """
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
@@ -38,6 +39,11 @@ class _PagedLayer(CacheLayerMixin):
 
     def update(self, key_states, value_states, *args, **kwargs):
         c = self._cache
+        if c.handed is not None:
+            raise RuntimeError(
+                f"the keys that layer {c.handed} got from this cache did not reach the fa_p100 attention, and any other "
+                "would see the newest tokens alone: call enable_fa_p100 on the model (or, if that call failed, "
+                "reset the cache)")
         B, heads, N, D = key_states.shape
         if self._tokens and N > 1:              # before anything is stored
             raise NotImplementedError(
@@ -57,7 +63,12 @@ class _PagedLayer(CacheLayerMixin):
         # a tensor of its own to carry the mark: the caller's may serve elsewhere
         key_states = key_states.view_as(key_states)
         key_states._fa_p100_paged = (self, past)
+        c.handed = self._index
         return key_states, value_states
+
+    def reached(self):
+        """The attention call has this layer's keys."""
+        self._cache.handed = None
 
     def attention(self, query):
         """(B, 1, Hq, D) of the queries (B, Hq, 1, D) of the newest tokens."""
@@ -95,6 +106,7 @@ class FaP100Cache(Cache):
         if max_len < 1 or page_size < 1:
             raise RuntimeError("max_len and page_size must be positive")
         self.batch, self.tokens = batch, 0
+        self.handed = None      # the layer whose keys are on their way to its attention call
         # a full row of pages for every sequence: no request is ever refused
         pages = batch * -(-max_len // page_size)
         self.paged = PagedKVCache(layers, kv_heads, head_dim, pages, batch, max_len, page_size, dtype, device)
@@ -112,6 +124,6 @@ class FaP100Cache(Cache):
         """Empties the cache for another batch of prompts."""
         if self.tokens:
             self.paged.release(torch.ones(self.batch, dtype=torch.bool, device=self.paged.lens.device))
-        self.tokens = 0
+        self.tokens, self.handed = 0, None
         for layer in self.layers:
             layer.reset()

@@ -257,3 +257,31 @@ def test_hf_cache_refuses_a_second_prompt_unchanged(monkeypatch):
         assert calls == ["extend", "append", "append"] and cache.tokens == 5 and cache.get_seq_length() == 5
         model(ids(1), past_key_values=cache, use_cache=True)
     assert calls[3:] == ["extend", "append", "attn", "append", "attn"] and cache.get_seq_length() == 6
+
+
+def test_hf_cache_refuses_another_attention(monkeypatch):
+    """The cache hands on the new keys alone, which only the fa_p100 attention can
+    complete: under sdpa a decoding step would see one token, without a word."""
+    model = hf_model(impl="sdpa")
+    cache, calls = hf_cache(model, monkeypatch)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="enable_fa_p100"):
+        model(ids(5), past_key_values=cache, use_cache=True)
+    assert calls == ["extend", "append"]
+    cache.reset()
+    model = hf_model(layers=1, impl="sdpa")     # one layer: the second call shows it
+    cache, calls = hf_cache(model, monkeypatch)
+    with torch.no_grad():
+        model(ids(5), past_key_values=cache, use_cache=True)
+        with pytest.raises(RuntimeError, match="enable_fa_p100"):
+            model(ids(1), past_key_values=cache, use_cache=True)
+    # reset, and a model that has it
+    cache.reset()
+    model = hf_model(layers=1)
+    with torch.no_grad():
+        for n in (5, 1, 1):
+            model(ids(n), past_key_values=cache, use_cache=True)
+    assert cache.get_seq_length() == 7
+    # a call that the attention refuses does not count as lost
+    with torch.no_grad(), pytest.raises(NotImplementedError, match="head_mask"):
+        model(ids(1), past_key_values=cache, use_cache=True, head_mask=torch.ones(2))
+    assert cache.handed is None

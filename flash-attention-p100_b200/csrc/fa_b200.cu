@@ -58,6 +58,7 @@ struct DeviceState {
   int status = FA_B200_OK;
   int* err = nullptr;  // address of g_device_error on this device
   int sms = 148;       // multiprocessors
+  int cluster = 16;    // most blocks of a paged attention's cluster
 };
 
 std::mutex g_mu;
@@ -124,9 +125,27 @@ void set_smem_all() {
   set_smem(paged_join_kernel<128, BF>, 0);
 }
 
+// Clusters of 16 blocks (beyond the portable 8) need a GPC with as many SMs to itself,
+// which a context with a part of the GPU may not have.
+int most_cluster() {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 16;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(16);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = PagedCfg<128>::SMEM;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  const bool asked = cudaOccupancyMaxActiveClusters(&clusters, paged_attn_kernel<128, true, 32, true>, &cfg) == cudaSuccess;
+  return asked && clusters > 0 ? 16 : 8;
+}
+
 // One-time, per-device set-up with that device current: architecture check,
 // opt-in to large dynamic shared memory, and the error word's address.
-int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr) {
+int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr, int* cluster_out = nullptr) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return FA_B200_ERR_DEVICE;
   // Bind the device's primary context to this host thread. The tensor-map
@@ -164,12 +183,17 @@ int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr) {
         set_smem(release_fill_kernel, 0);
         set_smem(append_kernel<64>, 0), set_smem(append_kernel<128>, 0);
         st.status = (cudaGetLastError() == cudaSuccess) ? FA_B200_OK : FA_B200_ERR_DEVICE;
+        if (st.status == FA_B200_OK) {
+          st.cluster = most_cluster();
+          (void)cudaGetLastError();   // not this set-up's
+        }
       }
     }
     st.ready = true;
   }
   *err_out = st.err;
   if (sms_out) *sms_out = st.sms;
+  if (cluster_out) *cluster_out = st.cluster;
   return st.status;
 }
 
@@ -286,30 +310,6 @@ bool to_units(const Strides& s, int P, int Hkv, Units* u) {
   return true;
 }
 
-// Blocks of a cluster for `units` units whose table rows hold up to `most` steps
-// (32 KB of cache each), 0 where the line is used. Clusters need all their blocks
-// at once: two blocks an SM, one for clusters of 16, which fill a GPC. The line
-// keeps every SM busy whatever the lengths, but adds them up first and joins in a
-// second launch. Device time of a call, clusters / line, in us (bf16):
-//   8 kv heads, D=128, 1 request:    512 tokens 4.6 / 7.1, 2048 6.7 / 7.8, 8192 12.3 / 10.7
-//   32 requests of 512 tokens 11.0 / 14.7, of 1 to 512 10.3 / 13.2, of 1 to 1024 16.2 / 18.5
-//   20 requests (160 blocks) of 512 tokens 10.7 / 12.7, of 1024 17.4 / 16.5
-//   40 requests (two blocks a unit, in waves) of 256 tokens 14.9 / 12.9
-//   1 kv head, D=64, 1 request: 2048 tokens 5.1 / 6.6, 8192 7.7 / 7.0, 16000 13.2 / 8.4
-//   256 units (a block each), D=64, 2048 tokens 25.1 / 28.8, of 1 to 2048 19.2 / 16.8
-// so the steps a block may have to take grow with the part of the GPU in use, where
-// a unit's keys are spread over several blocks.
-int paged_cluster(long long units, long long most, int sms) {
-  for (int c = 16; c >= 1; c /= 2) {
-    const long long blocks = units * c;
-    if (c > 1 && c / 2 >= most) continue;   // no more blocks than steps
-    if (blocks > (c == 16 ? sms : 2 * sms)) continue;
-    const int steps = c > 1 && 2 * blocks > 3 * sms ? 16 : 2 * blocks > sms ? 8 : 4;
-    return most <= static_cast<long long>(c) * steps ? c : 0;
-  }
-  return 0;
-}
-
 // How a call is cut: query heads of a row tile, units, steps of a full row, blocks
 // of a cluster (0: the line) and blocks of the launch.
 struct PagedPlan {
@@ -317,7 +317,7 @@ struct PagedPlan {
   long long units, most, blocks;
 };
 
-PagedPlan paged_plan(int B, int Hq, int Hkv, int W, int D, int page, int sms) {
+PagedPlan paged_plan(int B, int Hq, int Hkv, int W, int D, int page, int sms, int max_cluster) {
   const int group = Hq / Hkv;
   PagedPlan p{};
   const auto cut = [&](int rows, int step) {
@@ -330,7 +330,7 @@ PagedPlan paged_plan(int B, int Hq, int Hkv, int W, int D, int page, int sms) {
     p.blocks = static_cast<long long>(std::min<double>(blocks, static_cast<double>(p.units) * p.most));
   };
   cut(group <= 8 ? 8 : group <= 16 ? 16 : 32, D == 64 ? PagedCfg<64>::STEP : PagedCfg<128>::STEP);
-  p.cluster = paged_cluster(p.units, p.most, sms);
+  p.cluster = paged_cluster(p.units, p.most, sms, max_cluster);
   if (p.cluster) {
     p.blocks = p.units * p.cluster;
   } else if (group <= kPagedWarpHeads) {
@@ -1134,10 +1134,10 @@ int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b2
 
 size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, int page_size) {
   if (fab::check_shape(B, Hq, Hkv, 1, D) || fab::check_pages(1, W, page_size)) return 0;
-  int dev = 0, sms = 0;
+  int dev = 0, sms = 0, cluster = 0;
   int* err = nullptr;
-  if (fab::device_setup(&dev, &err, &sms) != FA_B200_OK) return 0;
-  return fab::paged_workspace(fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms), Hq / Hkv, D);
+  if (fab::device_setup(&dev, &err, &sms, &cluster) != FA_B200_OK) return 0;
+  return fab::paged_workspace(fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms, cluster), Hq / Hkv, D);
 }
 
 int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, fa_b200_strides skc,
@@ -1169,9 +1169,9 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
       !fab::strides_ok(a.so, 2) || !fab::strides_ok(sk, 2) || !fab::strides_ok(sv, 2))
     return FA_B200_ERR_ALIGNMENT;
   if (!fab::to_units(sk, P, Hkv, &a.skc) || !fab::to_units(sv, P, Hkv, &a.svc)) return FA_B200_ERR_TOO_LARGE;
-  int dev = 0, sms = 0;
-  if (int st = fab::device_setup(&dev, &a.err, &sms)) return st;
-  const fab::PagedPlan plan = fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms);
+  int dev = 0, sms = 0, cluster = 0;
+  if (int st = fab::device_setup(&dev, &a.err, &sms, &cluster)) return st;
+  const fab::PagedPlan plan = fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms, cluster);
   const size_t need = fab::paged_workspace(plan, Hq / Hkv, D);
   if (need && (!workspace || workspace_bytes < need)) return FA_B200_ERR_WORKSPACE;
   const bool bf = dtype == FA_B200_DTYPE_BF16;

@@ -432,6 +432,31 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // line is paged_wide_kernel's: two fragments' products at 8 warps an SM are bound by
 // their latency, 85 us at 32 heads. Clusters take them here, up to 32 heads a tile.
 
+// Blocks of a cluster for `units` units whose table rows hold up to `most` steps
+// (32 KB of cache each), 0 where the line is used. Clusters need all their blocks
+// at once: two blocks an SM, one for clusters of 16, which fill a GPC. The line
+// keeps every SM busy whatever the lengths, but adds them up first and joins in a
+// second launch. A cluster has up to `max_cluster` blocks, which the device can place.
+// Device time of a call, clusters / line, in us (bf16):
+//   8 kv heads, D=128, 1 request:    512 tokens 4.6 / 7.1, 2048 6.7 / 7.8, 8192 12.3 / 10.7
+//   32 requests of 512 tokens 11.0 / 14.7, of 1 to 512 10.3 / 13.2, of 1 to 1024 16.2 / 18.5
+//   20 requests (160 blocks) of 512 tokens 10.7 / 12.7, of 1024 17.4 / 16.5
+//   40 requests (two blocks a unit, in waves) of 256 tokens 14.9 / 12.9
+//   1 kv head, D=64, 1 request: 2048 tokens 5.1 / 6.6, 8192 7.7 / 7.0, 16000 13.2 / 8.4
+//   256 units (a block each), D=64, 2048 tokens 25.1 / 28.8, of 1 to 2048 19.2 / 16.8
+// so the steps a block may have to take grow with the part of the GPU in use, where
+// a unit's keys are spread over several blocks.
+__host__ constexpr int paged_cluster(long long units, long long most, int sms, int max_cluster) {
+  for (int c = max_cluster; c >= 1; c /= 2) {
+    const long long blocks = units * c;
+    if (c > 1 && c / 2 >= most) continue;   // no more blocks than steps
+    if (blocks > (c == 16 ? sms : 2 * sms)) continue;
+    const int steps = c > 1 && 2 * blocks > 3 * sms ? 16 : 2 * blocks > sms ? 8 : 4;
+    return most <= static_cast<long long>(c) * steps ? c : 0;
+  }
+  return 0;
+}
+
 // Strides of a cache in units of 16 bytes (page, head, token): 32 bits each, so a
 // stride may be 64 GB, and one instruction for each product, which has 64.
 struct Units {

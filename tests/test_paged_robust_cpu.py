@@ -285,3 +285,26 @@ def test_hf_cache_refuses_another_attention(monkeypatch):
     with torch.no_grad(), pytest.raises(NotImplementedError, match="head_mask"):
         model(ids(1), past_key_values=cache, use_cache=True, head_mask=torch.ones(2))
     assert cache.handed is None
+
+
+def test_no_cluster_is_larger_than_the_device_can_place(tmp_path):
+    """One kv head or eight, short tables to long, on a whole B200 and on a context of
+    fewer SMs, with and without room for clusters of 16."""
+    checks = []
+    for units in (1, 2, 8, 9, 18, 37, 74, 148, 296, 297):
+        for most in (1, 2, 5, 16, 64, 128, 129, 1 << 20):
+            for sms in (148, 74, 18, 8):
+                for top in (16, 8):
+                    checks.append(f"static_assert(sane(fab::paged_cluster({units}, {most}, {sms}, {top}), {units}, {most}, "
+                                  f"{sms}, {top}));")
+    ok, err = compiles(tmp_path, """
+#include <cuda.h>
+#include "fa_paged.cuh"
+// none, or a power of two up to the top whose blocks are on the GPU at once
+constexpr bool sane(int c, long long units, long long most, int sms, int top) {
+  return c == 0 || (c > 0 && c <= top && (c & (c - 1)) == 0 && units * c <= (c == 16 ? sms : 2 * sms) && most <= 16ll * c);
+}
+static_assert(fab::paged_cluster(8, 64, 148, 16) == 16 && fab::paged_cluster(8, 64, 148, 8) == 0);
+static_assert(fab::paged_cluster(8, 32, 148, 16) == 16 && fab::paged_cluster(8, 32, 148, 8) == 8);
+""" + "\n".join(checks))
+    assert ok, err

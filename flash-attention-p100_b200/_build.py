@@ -24,6 +24,9 @@ DEBUG_LIB_PATH = os.path.join(HERE, "libfa_b200_debug.so")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
+    # nvcc compresses device code of this size (12 MB to 4), and the first call of every
+    # process unpacks it: 17 ms against 12
+    "--no-compress",
     "-Xcompiler", "-fPIC", "-shared",
 ]
 

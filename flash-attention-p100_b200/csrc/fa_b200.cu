@@ -58,6 +58,8 @@ struct DeviceState {
   int status = FA_B200_OK;
   int* err = nullptr;  // address of g_device_error on this device
   int sms = 148;       // multiprocessors
+  bool paged_ready = false;   // the paged kernels' own set-up (paged_setup)
+  int paged_status = FA_B200_OK;
   int cluster = 16;    // most blocks of a paged attention's cluster
 };
 
@@ -111,6 +113,9 @@ void set_smem_all() {
   set_smem(bwd_dq_kernel<128, BF>, DqCfg<128>::SMEM);
   set_smem(bwd_fused_kernel<64, BF>, FusedCfg<64>::SMEM);
   set_smem(bwd_fused_kernel<128, BF>, FusedCfg<128>::SMEM);
+}
+template <bool BF>
+void set_smem_paged_all() {
   set_smem_paged<64, BF, 8>();
   set_smem_paged<64, BF, 16>();
   set_smem_paged<64, BF, 32>();
@@ -145,7 +150,7 @@ int most_cluster() {
 
 // One-time, per-device set-up with that device current: architecture check,
 // opt-in to large dynamic shared memory, and the error word's address.
-int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr, int* cluster_out = nullptr) {
+int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return FA_B200_ERR_DEVICE;
   // Bind the device's primary context to this host thread. The tensor-map
@@ -177,24 +182,40 @@ int device_setup(int* dev_out, int** err_out, int* sms_out = nullptr, int* clust
         st.err = static_cast<int*>(addr);
         set_smem_all<false>();
         set_smem_all<true>();
-        // loads the paged kernels that need no opt-in: a first call may be captured
-        set_smem(extend_kernel, 0), set_smem(extend_fill_kernel, 0);
-        set_smem(release_kernel<true>, 0), set_smem(release_kernel<false>, 0);
-        set_smem(release_fill_kernel, 0);
-        set_smem(append_kernel<64>, 0), set_smem(append_kernel<128>, 0);
         st.status = (cudaGetLastError() == cudaSuccess) ? FA_B200_OK : FA_B200_ERR_DEVICE;
-        if (st.status == FA_B200_OK) {
-          st.cluster = most_cluster();
-          (void)cudaGetLastError();   // not this set-up's
-        }
       }
     }
     st.ready = true;
   }
   *err_out = st.err;
   if (sms_out) *sms_out = st.sms;
-  if (cluster_out) *cluster_out = st.cluster;
   return st.status;
+}
+
+// device_setup, and once more what the paged kernels need. They are not loaded with the
+// others, which made the first flash_attn call of a process 2 ms longer.
+// All of them are loaded here, also those that need no opt-in, so that a first call may
+// be captured.
+int paged_setup(int* dev_out, int** err_out, int* sms_out = nullptr, int* cluster_out = nullptr) {
+  if (int st = device_setup(dev_out, err_out, sms_out)) return st;
+  std::lock_guard<std::mutex> lock(g_mu);
+  DeviceState& st = g_dev[*dev_out];
+  if (!st.paged_ready) {
+    set_smem_paged_all<false>();
+    set_smem_paged_all<true>();
+    set_smem(extend_kernel, 0), set_smem(extend_fill_kernel, 0);
+    set_smem(release_kernel<true>, 0), set_smem(release_kernel<false>, 0);
+    set_smem(release_fill_kernel, 0);
+    set_smem(append_kernel<64>, 0), set_smem(append_kernel<128>, 0);
+    st.paged_status = (cudaGetLastError() == cudaSuccess) ? FA_B200_OK : FA_B200_ERR_DEVICE;
+    if (st.paged_status == FA_B200_OK) {
+      st.cluster = most_cluster();
+      (void)cudaGetLastError();   // not this set-up's
+    }
+    st.paged_ready = true;
+  }
+  if (cluster_out) *cluster_out = st.cluster;
+  return st.paged_status;
 }
 
 // 3-D fp16 (or fp32) tensor (slices, rows, cols) with 128-byte swizzled boxes
@@ -1056,7 +1077,7 @@ int fa_b200_paged_extend(const int* new_lens, const int* lens, int* block_table,
   if (!fab::aligned16(workspace)) return FA_B200_ERR_ALIGNMENT;
   int dev = 0, sms = 0;
   int* err = nullptr;
-  if (int st = fab::device_setup(&dev, &err, &sms)) return st;
+  if (int st = fab::paged_setup(&dev, &err, &sms)) return st;
   auto* head = static_cast<fab::TableHead*>(workspace);
   const fab::ExtendArgs a{new_lens, lens, free_pages, free_count, block_table, slots, granted,
                           lens_out, free_count_out, table_stride, head,
@@ -1087,7 +1108,7 @@ int fa_b200_paged_release(const unsigned char* finished, const int* lens, const 
   if (!fab::aligned16(workspace)) return FA_B200_ERR_ALIGNMENT;
   int dev = 0, sms = 0;
   int* err = nullptr;
-  if (int st = fab::device_setup(&dev, &err, &sms)) return st;
+  if (int st = fab::paged_setup(&dev, &err, &sms)) return st;
   auto* head = static_cast<fab::TableHead*>(workspace);
   const fab::ReleaseArgs a{finished, lens, block_table, free_count, free_pages, lens_out,
                            free_count_out, table_stride, head,
@@ -1127,7 +1148,7 @@ int fa_b200_paged_append(const void* k, fa_b200_strides sk, const void* v, fa_b2
   if (T == 0) return FA_B200_OK;
   int dev = 0;
   int* err = nullptr;
-  if (int st = fab::device_setup(&dev, &err)) return st;
+  if (int st = fab::paged_setup(&dev, &err)) return st;
   return fab::launch_after(D == 64 ? fab::append_kernel<64> : fab::append_kernel<128>, "append_kernel",
                            static_cast<unsigned>(blocks), 256, 0, 0, stream, a);
 }
@@ -1136,7 +1157,7 @@ size_t fa_b200_paged_attn_workspace_bytes(int B, int Hq, int Hkv, int W, int D, 
   if (fab::check_shape(B, Hq, Hkv, 1, D) || fab::check_pages(1, W, page_size)) return 0;
   int dev = 0, sms = 0, cluster = 0;
   int* err = nullptr;
-  if (fab::device_setup(&dev, &err, &sms, &cluster) != FA_B200_OK) return 0;
+  if (fab::paged_setup(&dev, &err, &sms, &cluster) != FA_B200_OK) return 0;
   return fab::paged_workspace(fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms, cluster), Hq / Hkv, D);
 }
 
@@ -1170,7 +1191,7 @@ int fa_b200_paged_attn(const void* q, fa_b200_strides sq, const void* k_cache, f
     return FA_B200_ERR_ALIGNMENT;
   if (!fab::to_units(sk, P, Hkv, &a.skc) || !fab::to_units(sv, P, Hkv, &a.svc)) return FA_B200_ERR_TOO_LARGE;
   int dev = 0, sms = 0, cluster = 0;
-  if (int st = fab::device_setup(&dev, &a.err, &sms, &cluster)) return st;
+  if (int st = fab::paged_setup(&dev, &a.err, &sms, &cluster)) return st;
   const fab::PagedPlan plan = fab::paged_plan(B, Hq, Hkv, W, D, page_size, sms, cluster);
   const size_t need = fab::paged_workspace(plan, Hq / Hkv, D);
   if (need && (!workspace || workspace_bytes < need)) return FA_B200_ERR_WORKSPACE;

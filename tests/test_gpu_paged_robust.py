@@ -1,7 +1,10 @@
 """The paged cache's operators where they can go wrong: many requests to wide groups,
 rows with nothing left, what autograd is told, memory that overlaps. The scenes and
 bounds are those of test_gpu_paged.py."""
+import os
 import random
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -167,3 +170,31 @@ def test_transforms_and_fake_tensors_are_refused(cuda):
             op(**{n: mode.from_tensor(t) for n, t in args.items()})
     torch.cuda.synchronize()
     assert torch.equal(a["k_cache"], kept[0]) and torch.equal(a["v_cache"], kept[1])
+
+
+def test_the_paged_kernels_are_loaded_by_their_own_first_call():
+    """In a process of its own: flash_attn's first call does not wait for them."""
+    code = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+import fa_p100, fa_p100_paged as paged
+dev = torch.device("cuda", 0)
+q = torch.randn(1, 4, 256, 64, device=dev).half()
+lens = torch.zeros(1, dtype=torch.int32, device=dev)
+a = (lens, lens, torch.zeros(1, 2, dtype=torch.int32, device=dev), lens, lens, 16, 1)
+torch.empty(1 << 20, device=dev), torch.empty(1 << 26, device=dev)     # torch's own pools
+free = lambda: (torch.cuda.synchronize(), torch.cuda.mem_get_info(dev)[0])[1]
+at = [free()]
+fa_p100.flash_attn(q, q, q, True)
+at.append(free())
+paged.paged_extend(*a)
+at.append(free())
+paged.paged_extend(*a)
+at.append(free())
+print(at[0] - at[1], at[1] - at[2], at[2] - at[3])
+"""
+    res = subprocess.run([sys.executable, "-c", code, os.path.dirname(paged.__file__)], capture_output=True, text=True,
+                         timeout=300)
+    assert res.returncode == 0, res.stderr[-2000:]
+    first, own, again = map(int, res.stdout.split())
+    assert first > 0 and own > 0 and again == 0

@@ -308,3 +308,8 @@ static_assert(fab::paged_cluster(8, 64, 148, 16) == 16 && fab::paged_cluster(8, 
 static_assert(fab::paged_cluster(8, 32, 148, 16) == 16 && fab::paged_cluster(8, 32, 148, 8) == 8);
 """ + "\n".join(checks))
     assert ok, err
+
+
+def test_the_library_is_not_unpacked_by_every_process():
+    """Compressed device code is a third of the size and costs each first call."""
+    assert "--no-compress" in _build.NVCC_FLAGS

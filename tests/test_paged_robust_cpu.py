@@ -109,7 +109,7 @@ def slices(name):
     return {
         "next to each other": ((view(0, *head), view(4 * page, *head)), False),
         "last page and first": ((view(0, *head), view(3 * page, *head)), True),
-        "heads 0-1 and 1-2 of 3": ((view(0, 3072, 1024, 64, 1), view(1024, 3072, 1024, 64, 1)), True),
+        "heads 0-1 and 1-2 of 5": ((view(0, 5120, 1024, 64, 1), view(1024, 5120, 1024, 64, 1)), True),
         "heads 0-1 and 2-3 of 4": ((view(0, 4096, 1024, 64, 1), view(2048, 4096, 1024, 64, 1)), False),
         "pages in turn": ((view(0, 2 * page, 1024, 64, 1), view(page, 2 * page, 1024, 64, 1)), False),
         "pages in turn, a row over": ((view(0, 2 * page, 1024, 64, 1), view(page - 64, 2 * page, 1024, 64, 1)), True),
@@ -125,7 +125,7 @@ def slices(name):
 
 
 @pytest.mark.parametrize("name", [
-    "next to each other", "last page and first", "heads 0-1 and 1-2 of 3", "heads 0-1 and 2-3 of 4", "pages in turn",
+    "next to each other", "last page and first", "heads 0-1 and 1-2 of 5", "heads 0-1 and 2-3 of 4", "pages in turn",
     "pages in turn, a row over", "by token, k and v in turn", "by token, one head over", "rows in turn", "half a row",
     "page's first 8 bytes", "two layouts apart", "two layouts over", "two layouts in turn"])
 def test_append_refuses_caches_that_share_memory(name):

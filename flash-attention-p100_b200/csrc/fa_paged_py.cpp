@@ -169,16 +169,24 @@ bool makes_up(const Axis* axis, const Axis* end, int64_t distance, int& budget) 
     if (--budget < 0 || makes_up(axis + 1, end, distance - i * axis->stride, budget)) return true;
   return false;
 }
-bool share_memory(const at::Tensor& a, const at::Tensor& b) {
-  if (a.numel() == 0 || b.numel() == 0) return false;
-  const auto bytes = [](const at::Tensor& t) {   // from the first element to behind the last
-    int64_t n = t.element_size();
-    for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i) * t.element_size();
-    return n;
-  };
-  const int64_t distance =
-      static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()) - reinterpret_cast<uintptr_t>(a.data_ptr()));
-  if (distance >= bytes(a) || -distance >= bytes(b)) return false;
+
+// The bytes from a tensor's first element to behind its last: most tensors are told
+// apart by these alone.
+struct Span {
+  const at::Tensor& t;
+  uintptr_t first;
+  int64_t bytes;   // 0 without an element
+  explicit Span(const at::Tensor& x) : t(x), first(reinterpret_cast<uintptr_t>(x.const_data_ptr())) {
+    const auto sizes = x.sizes(), strides = x.strides();
+    int64_t last = 0;
+    for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+    bytes = x.numel() == 0 ? 0 : (last + 1) * static_cast<int64_t>(x.itemsize());
+  }
+};
+bool share_memory(const Span& sa, const Span& sb) {
+  const auto distance = static_cast<int64_t>(sb.first - sa.first);
+  if (sa.bytes == 0 || sb.bytes == 0 || distance >= sa.bytes || -distance >= sb.bytes) return false;
+  const at::Tensor &a = sa.t, &b = sb.t;
   Axis axes[16];   // the tensors have up to 4 axes each
   int n = 0;
   const auto add = [&](int64_t stride, int64_t lo, int64_t hi) {
@@ -376,9 +384,11 @@ void append(pybind11::handle k_new, pybind11::handle v_new, pybind11::handle slo
   for (const fa_b200_strides& st : {c.sk, c.sv})
     if (st.batch == 0 || st.head == 0 || st.row == 0)
       refuse("k_cache and v_cache are written and must not be expanded views");
-  if (share_memory(c.k, c.v)) refuse("k_cache and v_cache must be different memory");
+  const Span in_k(c.k), in_v(c.v);
+  if (share_memory(in_k, in_v)) refuse("k_cache and v_cache must be different memory");
   for (const Named& x : {Named{"k", k}, Named{"v", v}, Named{"slots", s}})
-    if (share_memory(x.t, c.k) || share_memory(x.t, c.v)) refuse(x.name, " must not overlap the caches");
+    if (const Span span(x.t); share_memory(span, in_k) || share_memory(span, in_v))
+      refuse(x.name, " must not overlap the caches");
   no_grad({{"k", k}, {"v", v}, {"k_cache", c.k}, {"v_cache", c.v}});
   Call call(one_device({{"k_cache", c.k}, {"v_cache", c.v}, {"k", k}, {"v", v}, {"slots", s}}));
   if (T == 0) return;

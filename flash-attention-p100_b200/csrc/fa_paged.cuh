@@ -179,7 +179,10 @@ __device__ __forceinline__ bool extend_rows(const ExtendArgs& a) {
 // threads `first`, `first + step`, ... of the launch. New entries lie behind
 // the entries that this reads (a request's pages so far), so the order of the
 // threads does not matter. A thread takes kSlotRun tokens in a row: one search
-// and, inside a request, at most two pages (a page holds 16 or more).
+// and, inside a request, at most two pages (a page holds 16 or more). A run that meets
+// a request's end steps over the requests behind it one by one: 5001 tokens of one
+// request take 5.2 us alone, 9.1 ahead of 63 requests without new tokens, 20 of 255 and
+// 122 of 2047.
 constexpr int kSlotRun = 8;
 constexpr int kRowsShared = 2048;  // rows whose first tokens and pages are searched in shared memory
 
@@ -424,11 +427,11 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 // (cp.async, 16 bytes a lane), three steps deep, across unit borders too: the
 // loads never drain, and warps meet only where a unit ends.
 //
-// Measured: 64 ragged requests of 32/8 heads of 128 (1.0 GB of cache) 155 us, 6.45
-// TB/s or 98% of the measured copy, DRAM traffic equal to the cache's bytes, a fifth
-// of the tensor pipe; one request of 131001 tokens 85 us, 6.3 TB/s; one of 1000
-// tokens 6.0 us, a chain of dependent loads (length, page, keys). 16 heads
-// for 32 sequences of 4096 tokens, 0.27 GB: 52 us, 5.2 TB/s. Wider groups'
+// Measured: 64 ragged requests of 32/8 heads of 128 (1.0 GB of cache) 154 to 158 us,
+// 6.3 to 6.5 TB/s or 97 to 99% of the measured copy, DRAM traffic equal to the cache's
+// bytes, a fifth of the tensor pipe; one request of 131001 tokens 85 us, 6.3 TB/s; one
+// of 1000 tokens 6.0 us, a chain of dependent loads (length, page, keys). 16 heads
+// for 32 sequences of 4096 tokens, 0.27 GB: 54 us, 5.0 TB/s. Wider groups'
 // line is paged_wide_kernel's: two fragments' products at 8 warps an SM are bound by
 // their latency, 85 us at 32 heads. Clusters take them here, up to 32 heads a tile.
 
@@ -444,8 +447,13 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
 //   40 requests (two blocks a unit, in waves) of 256 tokens 14.9 / 12.9
 //   1 kv head, D=64, 1 request: 2048 tokens 5.1 / 6.6, 8192 7.7 / 7.0, 16000 13.2 / 8.4
 //   256 units (a block each), D=64, 2048 tokens 25.1 / 28.8, of 1 to 2048 19.2 / 16.8
+//   64 units (four blocks each), D=64, 2048 tokens 8.2 / 11.6, 8192 25.7 / 28.7, of 1 to
+//   8192 19.3 / 15.7; D=128, 2048 tokens 11.2 / 14.3, 4096 24.9 / 28.4, of 1 to 4096 16.7 / 15.2
 // so the steps a block may have to take grow with the part of the GPU in use, where
-// a unit's keys are spread over several blocks.
+// a unit's keys are spread over several blocks. Lengths are not known here, so the rule
+// goes by the rows of the table and has a wrong side: full rows at its borders (8192
+// tokens above), ragged ones in long rows, and 72 to 74 units, whose clusters of four
+// do not all find a place at once (74 units, D=64, 1024 tokens 9.3 / 8.2, 8192 42 / 31).
 __host__ constexpr int paged_cluster(long long units, long long most, int sms, int max_cluster) {
   for (int c = max_cluster; c >= 1; c /= 2) {
     const long long blocks = units * c;

@@ -193,8 +193,13 @@ paged.paged_extend(*a)
 at.append(free())
 print(at[0] - at[1], at[1] - at[2], at[2] - at[3])
 """
-    res = subprocess.run([sys.executable, "-c", code, os.path.dirname(paged.__file__)], capture_output=True, text=True,
-                         timeout=300)
-    assert res.returncode == 0, res.stderr[-2000:]
-    first, own, again = map(int, res.stdout.split())
-    assert first > 0 and own > 0 and again == 0
+    seen = []
+    for _ in range(3):      # free memory is the whole GPU's: another process may move it
+        res = subprocess.run([sys.executable, "-c", code, os.path.dirname(paged.__file__)], capture_output=True,
+                             text=True, timeout=300)
+        assert res.returncode == 0, res.stderr[-2000:]
+        first, own, again = map(int, res.stdout.split())
+        if first > 0 and own > 0 and again == 0:
+            return
+        seen.append((first, own, again))
+    assert False, f"bytes taken by the first flash_attn, the first paged call and the second: {seen}"
